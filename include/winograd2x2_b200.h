@@ -39,6 +39,9 @@ enum { WG2X2_NHWC = 0, WG2X2_NCHW = 1 };
  * WG2X2_MATH_TF32: tcgen05 kind::tf32 tensor-core MMAs accumulating in TMEM (<= 5e-3). */
 enum { WG2X2_MATH_FP32 = 0, WG2X2_MATH_TF32 = 1 };
 
+/* Element types of the 8-bit products' inputs and outputs (everything else here is fp32) */
+enum { WG2X2_F32 = 0, WG2X2_F16 = 1, WG2X2_BF16 = 2 };
+
 const char *wg2x2_status_string(int status);
 
 /* Version of this ABI (bumped when a signature changes). */
@@ -193,6 +196,39 @@ int wg2x2_conv1x1(const float *X, const float *W, float *Y, int B, int C, int K,
 int wg2x2_conv1x1_preferred(int B, int C, int K, int HW);
 
 /*
+ * Rows of 8-bit codes with one scale a row, the operands of wg2x2_linear_int8.  A row is a pixel (or token) with its C channels:
+ *     a = max_c |x_c|,  scale = a / 127,  Q_c = 127 x_c / a to the nearest whole number (ties to the even one, as in exact arithmetic)
+ * with x passed through a ReLU first where relu != 0.  A row whose a is below 2^-119 has scale 0 and codes 0; one with a NaN or an
+ * infinity has scale NaN and codes 0 (and so stays NaN in a product).
+ * X: B x HW pixels of `type` (WG2X2_F32 / F16 / BF16), WG2X2_NHWC: B*HW rows, ldx elements apart, or WG2X2_NCHW: (B,C,HW) dense (ldx is not
+ * read).  Q: B*HW rows of C signed bytes, ldq apart, in either layout; bytes of a row behind its C stay as they are.  scale: B*HW
+ * floats.  Any alignment that the types have; rows that begin on 16 bytes are faster.  B = 0 does nothing.  Weights (K,C) of a product
+ * go through the same call, with K rows.
+ */
+int wg2x2_quantize_int8(const void *X, int type, long long ldx, void *Q, long long ldq, float *scale, long long B, int HW, int C, int layout,
+                        int relu, void *stream);
+/*
+ * The same behind a root-mean-square norm over the channels, with a shortcut's addition in front:
+ *     h = X + residual, rounded to `type` and stored in residual_out;  u_c = h_c weight_c in 32 bits;  a = max_c |u_c|
+ *     scale = a / 127 / sqrt(mean_c h_c^2 + eps),  Q_c = 127 u_c / a as above
+ * residual and residual_out (both or neither NULL) have X's type and layout, with row pitches ldr and ldo; residual_out may lie exactly
+ * over X or over residual.  weight: C values of `type`, or floats where weight_f32 != 0.  eps at least 1e-30.  The squares are added in
+ * 32 bits; rows whose squares leave 32 bits are scaled.
+ */
+int wg2x2_rms_norm_int8(const void *X, long long ldx, const void *residual, long long ldr, void *residual_out, long long ldo, const void *weight,
+                        int weight_f32, float eps, int type, void *Q, long long ldq, float *scale, long long B, int HW, int C, int layout,
+                        void *stream);
+/*
+ * Product of codes, Y[r][k] = (sum_c Q[r][c] W[k][c]) * w_scale[k] * q_scale[r] (+ bias[k]), through a ReLU where relu != 0 (NaN stays), on
+ * the tensor cores.  The sum is exact; what follows is in 32 bits, rounded once to `type`.  Q: B*HW rows of C signed bytes ldq apart, W: K
+ * rows ldw apart, rows on 16-byte boundaries (WG2X2_ERR_BAD_ARG otherwise); bytes behind a row's C are not used.  bias: K floats or
+ * NULL.  Y: WG2X2_NHWC, B*HW rows of K values ldy elements apart, or WG2X2_NCHW, (B,K,HW) dense (ldy is not read); it overlaps none of
+ * the operands.  C at most 131071 (WG2X2_ERR_UNSUPPORTED beyond): the sums then fit 32 bits.  No workspace.  B = 0 does nothing.
+ */
+int wg2x2_linear_int8(const void *Q, long long ldq, const float *q_scale, const void *W, long long ldw, const float *w_scale, const float *bias,
+                      int relu, void *Y, int type, long long ldy, long long B, int HW, int C, int K, int layout, void *stream);
+
+/*
  * out[p] = mean over the n values of plane p of relu(X): the ReLU and global average pool in front of the classifier
  * (ResNet-18-var/imagenet-resnet-transWino-prune.py:216-219).  X: planes x n floats.
  */
@@ -313,7 +349,7 @@ int wg2x2_last_device_status(void *stream, unsigned int *where);
 int wg2x2_set_wait_limit(long long polls);
 /*
  * Test hooks for the time-out path (they fault and hang nothing).  wg2x2_test_drop_load(n): in the next
- * launch of conv_fwd (row-walk), layer_fwd_fused or conv1x1, CTA 0's weight producer stops before its n-th load, so the
+ * launch of conv_fwd (row-walk), layer_fwd_fused, conv1x1 or linear_int8, CTA 0's (weight) producer stops before its n-th load, so the
  * MMA issuer's wait for that stage runs out; one-shot, n < 0 disarms.  wg2x2_test_wait_probe: a one-thread
  * kernel that waits `polls` polls on a barrier nobody arrives on and records `where`.
  */

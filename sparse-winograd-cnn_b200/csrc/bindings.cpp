@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -652,6 +653,277 @@ PyObject *py_conv1x1(WG_ARGS)
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------
+// Products in 8-bit integers.  Their tensors are rows: the last dimension, and all others as one where their strides allow that.
+// ---------------------------------------------------------------------------------------
+int type_of(at::ScalarType t)
+{
+    return t == at::kFloat ? WG2X2_F32 : t == at::kHalf ? WG2X2_F16 : t == at::kBFloat16 ? WG2X2_BF16 : -1;
+}
+Tensor arg_on(PyObject *o, const char *name, const Tensor *with, bool optional = false)
+{
+    if (optional && o == Py_None) return Tensor();
+    if (!THPVariable_Check(o) || !THPVariable_Unpack(o).is_cuda()) type_error(std::string(name) + " must be a CUDA tensor");
+    const Tensor &t = THPVariable_Unpack(o);
+    if (t.layout() != at::kStrided) type_error(std::string(name) + " must be a dense tensor");
+    if (with && t.device() != with->device()) value_error(std::string(name) + " must be on the same device as the other tensors");
+    return t;
+}
+Tensor arg_real(PyObject *o, const char *name, const Tensor *with, bool optional = false)
+{
+    const Tensor t = arg_on(o, name, with, optional);
+    if (t.defined() && type_of(t.scalar_type()) < 0) type_error(std::string(name) + " must be float32, float16 or bfloat16");
+    return t;
+}
+void want_type(const Tensor &t, at::ScalarType type, const char *name)
+{
+    if (t.defined() && t.scalar_type() != type) type_error(std::string(name) + " must be " + at::toString(type));
+}
+void want_shape(const Tensor &t, at::IntArrayRef shape, const char *name)
+{
+    if (t.defined() && t.sizes() != shape)
+        value_error(std::string(name) + " has shape " + shape_text(t.sizes()) + ", expected " + shape_text(shape));
+}
+void want_dense(const Tensor &t, const char *name)
+{
+    if (t.defined() && !t.is_contiguous()) value_error(std::string(name) + " must be contiguous");
+}
+// float32, dense, of this shape
+Tensor arg_floats(PyObject *o, at::IntArrayRef shape, const char *name, const Tensor &with, bool optional = false)
+{
+    const Tensor t = arg_on(o, name, &with, optional);
+    want_type(t, at::kFloat, name);
+    want_shape(t, shape, name);
+    want_dense(t, name);
+    return t;
+}
+
+struct RowView {
+    int64_t rows = 1, C = 0, ld = 0;
+    bool ok = true;             // the rows are a pitch of ld >= C apart, their elements side by side
+};
+RowView rows_of(const Tensor &t)
+{
+    RowView v;
+    const auto n = t.sizes(), s = t.strides();
+    const int last = (int)n.size() - 1;
+    v.C = n[last];
+    if (v.C > 1 && s[last] != 1) v.ok = false;
+    bool first = true;
+    int64_t next = 0;           // the stride that the dimension in front has to have
+    for (int d = last - 1; d >= 0; --d) {
+        v.rows *= n[d];
+        if (n[d] == 1) continue;
+        if (first) v.ld = s[d];
+        else if (s[d] != next) v.ok = false;
+        next = s[d] * n[d];
+        first = false;
+    }
+    if (first) v.ld = v.C;
+    if (v.ld < v.C) v.ok = false;
+    return v;
+}
+RowView need_rows(const Tensor &t, const char *name)
+{
+    const RowView v = rows_of(t);
+    if (v.rows && !v.ok) value_error(std::string(name) + " must be rows of a common pitch with their elements side by side");
+    return v;
+}
+std::vector<int64_t> leading(const Tensor &t) { return std::vector<int64_t>(t.sizes().begin(), t.sizes().end() - 1); }
+std::vector<int64_t> with_last(std::vector<int64_t> shape, int64_t n) { shape.push_back(n); return shape; }
+
+// Codes in rows that begin on 16 bytes, as the product takes them
+Tensor new_codes(const std::vector<int64_t> &lead, int64_t C, const Tensor &like)
+{
+    const std::vector<int64_t> shape = with_last(lead, C);
+    std::vector<int64_t> strides(shape.size(), 1);
+    int64_t s = (C + 15) / 16 * 16;
+    for (int d = (int)shape.size() - 2; d >= 0; --d) { strides[d] = s; s *= std::max<int64_t>(shape[d], 1); }
+    return Tensor(at::detail::empty_strided_cuda(shape, strides, at::kChar, like.device()));
+}
+Tensor arg_codes(PyObject *o, const char *name, const Tensor *with)
+{
+    const Tensor t = arg_on(o, name, with);
+    want_type(t, at::kChar, name);
+    if (t.dim() < 1) value_error(std::string(name) + " must have at least one dimension");
+    return t;
+}
+// The same codes in such rows: a copy where they are not
+Tensor aligned_codes(const Tensor &t)
+{
+    const RowView v = rows_of(t);
+    if (!v.rows || !v.C || (v.ok && (v.rows == 1 || v.ld % 16 == 0) && on16(t))) return t;
+    const Tensor c = new_codes(leading(t), t.size(-1), t);
+    c.copy_(t);
+    return c;
+}
+int64_t pitch16(const RowView &v) { return v.rows == 1 ? (v.C + 15) / 16 * 16 : v.ld; }
+
+// Rows of an activation tensor: its shape without the channels, and what the C ABI takes of it
+struct Acts {
+    std::vector<int64_t> lead;
+    int64_t B = 0, HW = 1, C = 0, ld = 0;
+};
+Acts acts_of(const Tensor &x, int layout, const char *name)
+{
+    Acts a;
+    if (layout == WG2X2_NCHW) {
+        const Img d = img_of(x, layout, name);
+        want_dense(x, name);
+        a.lead = {d.B, d.H, d.W};
+        a.B = d.B; a.HW = d.H * d.W; a.C = d.C; a.ld = d.C;
+        if (a.HW > 0x7fffffff) value_error(std::string(name) + ": too many pixels in an image");
+        if (!a.HW) a.B = 0, a.HW = 1;
+    } else {
+        if (x.dim() < 1) value_error(std::string(name) + " must have at least one dimension");
+        const RowView v = need_rows(x, name);
+        a.lead = leading(x);
+        a.B = v.rows; a.C = v.C; a.ld = v.ld;
+    }
+    if (a.C < 1 || a.C > 0x7fffffff) value_error(std::string(name) + " must have between 1 and 2^31 - 1 channels");
+    return a;
+}
+// out (codes) and scale_out of the caller
+void arg_outputs(PyObject *o, PyObject *s, const Acts &a, const Tensor &x, Tensor &q, Tensor &scale)
+{
+    q = arg_on(o, "out", &x, true);
+    want_type(q, at::kChar, "out");
+    want_shape(q, with_last(a.lead, a.C), "out");
+    if (q.defined()) need_rows(q, "out");
+    scale = arg_floats(s, a.lead, "scale_out", x, true);
+}
+void new_outputs(const Acts &a, const Tensor &x, Tensor &q, Tensor &scale)
+{
+    if (!q.defined()) q = new_codes(a.lead, a.C, x);
+    if (!scale.defined()) scale = new_float(a.lead, x);
+}
+PyObject *tuple_of(std::initializer_list<Tensor> ts)
+{
+    PyObject *t = PyTuple_New((Py_ssize_t)ts.size());
+    if (!t) throw python_error();
+    Py_ssize_t i = 0;
+    for (const Tensor &e : ts) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(e));
+    return t;
+}
+
+// x, relu, layout, out, scale_out
+PyObject *py_quantize_int8(WG_ARGS)
+{
+    HANDLE_TH_ERRORS
+    want(n, 5);
+    const Tensor x = arg_real(a[0], "x", nullptr);
+    const bool relu = arg_bool(a[1]);
+    const int layout = arg_int(a[2]);
+    const Acts d = acts_of(x, layout, "x");
+    Tensor q, scale;
+    arg_outputs(a[3], a[4], d, x, q, scale);
+    {
+        WG_NOGIL;
+        OnDevice on(x);
+        new_outputs(d, x, q, scale);
+        check(wg2x2_quantize_int8(x.data_ptr(), type_of(x.scalar_type()), d.ld, q.data_ptr(), pitch16(rows_of(q)), ptr(scale), d.B, (int)d.HW, (int)d.C,
+                                  layout, relu, on.stream),
+              "wg2x2_quantize_int8");
+    }
+    return tuple_of({q, scale});
+    END_HANDLE_TH_ERRORS
+}
+
+// x, weight, residual, eps, layout, out, scale_out, residual_out
+PyObject *py_rms_norm_int8(WG_ARGS)
+{
+    HANDLE_TH_ERRORS
+    want(n, 8);
+    const Tensor x = arg_real(a[0], "x", nullptr);
+    const int layout = arg_int(a[4]);
+    const Acts d = acts_of(x, layout, "x");
+    const Tensor w = arg_real(a[1], "weight", &x);
+    if (w.scalar_type() != at::kFloat) want_type(w, x.scalar_type(), "weight");
+    want_shape(w, {d.C}, "weight");
+    want_dense(w, "weight");
+    const Tensor res = arg_on(a[2], "residual", &x, true);
+    const double eps = PyFloat_AsDouble(a[3]);
+    if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+    Tensor h = arg_on(a[7], "residual_out", &x, true);
+    if (h.defined() && !res.defined()) value_error("residual_out needs a residual");
+    int64_t ldr = d.ld, ldh = d.ld;
+    for (const auto &[t, name, ld] : {std::make_tuple(&res, "residual", &ldr), std::make_tuple((const Tensor *)&h, "residual_out", &ldh)}) {
+        if (!t->defined()) continue;
+        want_type(*t, x.scalar_type(), name);
+        want_shape(*t, x.sizes(), name);
+        if (layout == WG2X2_NCHW) want_dense(*t, name);
+        else *ld = need_rows(*t, name).ld;
+    }
+    Tensor q, scale;
+    arg_outputs(a[5], a[6], d, x, q, scale);
+    {
+        WG_NOGIL;
+        OnDevice on(x);
+        new_outputs(d, x, q, scale);
+        if (res.defined() && !h.defined()) {
+            h = Tensor(at::detail::empty_cuda(x.sizes(), x.scalar_type(), x.device(), std::nullopt));
+            ldh = d.C;
+        }
+        check(wg2x2_rms_norm_int8(x.data_ptr(), d.ld, res.defined() ? res.data_ptr() : nullptr, ldr, h.defined() ? h.data_ptr() : nullptr, ldh,
+                                  w.data_ptr(), w.scalar_type() == at::kFloat, (float)eps, type_of(x.scalar_type()), q.data_ptr(),
+                                  pitch16(rows_of(q)), ptr(scale), d.B, (int)d.HW, (int)d.C, layout, on.stream),
+              "wg2x2_rms_norm_int8");
+    }
+    return res.defined() ? tuple_of({q, scale, h}) : tuple_of({q, scale});
+    END_HANDLE_TH_ERRORS
+}
+
+// q, scale, w, w_scale, bias, relu, layout, dtype, out
+PyObject *py_linear_int8(WG_ARGS)
+{
+    HANDLE_TH_ERRORS
+    want(n, 9);
+    const Tensor q = arg_codes(a[0], "q", nullptr);
+    const Tensor scale = arg_floats(a[1], leading(q), "scale", q);
+    const Tensor w = arg_codes(a[2], "w", &q);
+    if (w.dim() != 2 || w.size(1) != q.size(-1)) value_error("w must be (K, C) with the channels of q, got " + shape_text(w.sizes()));
+    const int64_t K = w.size(0), C = w.size(1);
+    if (K < 1 || C < 1 || K > 0x7fffffff || C > 0x7fffffff) value_error("w must have between 1 and 2^31 - 1 rows and channels");
+    const Tensor ws = arg_floats(a[3], {K}, "w_scale", q);
+    const Tensor bias = arg_floats(a[4], {K}, "bias", q, true);
+    const bool relu = arg_bool(a[5]);
+    const int layout = arg_int(a[6]);
+    if (!THPDtype_Check(a[7])) type_error("dtype must be a torch.dtype");
+    const at::ScalarType type = reinterpret_cast<THPDtype *>(a[7])->scalar_type;
+    if (type_of(type) < 0) type_error("dtype must be float32, float16 or bfloat16");
+    std::vector<int64_t> shape;
+    int64_t B = scale.numel(), HW = 1;
+    if (layout == WG2X2_NCHW) {
+        need_dims(q, 4, "q");
+        shape = {q.size(0), K, q.size(1), q.size(2)};
+        HW = q.size(1) * q.size(2);
+        B = q.size(0);
+        if (HW > 0x7fffffff) value_error("q: too many pixels in an image");
+        if (!HW) B = 0, HW = 1;
+    } else {
+        shape = with_last(leading(q), K);
+    }
+    Tensor y = arg_on(a[8], "out", &q, true);
+    want_type(y, type, "out");
+    want_shape(y, shape, "out");
+    int64_t ldy = K;
+    if (y.defined()) {
+        if (layout == WG2X2_NCHW) want_dense(y, "out");
+        else ldy = need_rows(y, "out").ld;
+    }
+    {
+        WG_NOGIL;
+        OnDevice on(q);
+        if (!y.defined()) y = Tensor(at::detail::empty_cuda(shape, type, q.device(), std::nullopt));
+        const Tensor qa = aligned_codes(q), wa = aligned_codes(w);
+        check(wg2x2_linear_int8(qa.data_ptr(), pitch16(rows_of(qa)), cptr(scale), wa.data_ptr(), pitch16(rows_of(wa)), cptr(ws), cptr(bias), relu,
+                                y.data_ptr(), type_of(type), ldy, B, (int)HW, (int)C, (int)K, layout, on.stream),
+              "wg2x2_linear_int8");
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 // x (B,C,H,W) -> (B,C): mean of relu(x) over the pixels
 PyObject *py_relu_mean(PyObject *, PyObject *o)
 {
@@ -806,6 +1078,9 @@ PyMethodDef methods[] = {
     WG_FN("residual_block", py_residual_block),
     WG_FN("conv1x1", py_conv1x1),
     {"relu_mean", py_relu_mean, METH_O, nullptr},
+    WG_FN("quantize_int8", py_quantize_int8),
+    WG_FN("rms_norm_int8", py_rms_norm_int8),
+    WG_FN("linear_int8", py_linear_int8),
     WG_FN("maxpool", py_maxpool),
     WG_FN("stem_pool", py_stem_pool),
     WG_FN("imtrans_op", py_imtrans_op),

@@ -15,6 +15,8 @@
 // Every mbarrier wait is bounded; on expiry the kernel records where it gave up, drains
 // and returns (status readable through wg2x2_last_device_status).
 #include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <atomic>
@@ -846,6 +848,7 @@ void dw_reduce_launch(const float *partial, const float *mask, float *dW, long l
 #include "conv_tc_pair.cuh"
 #include "stem_tc.cuh"
 #include "conv1x1_tc.cuh"
+#include "linear_int8.cuh"
 
 #if defined(WG_TC_TRACE) || defined(WG_TC_DIAG)   // development builds only
 extern "C" int wg2x2_debug_read_diag(unsigned int *host)
@@ -885,6 +888,13 @@ extern "C" int wg2x2_conv1x1_preferred(int B, int C, int K, int HW)
 extern "C" int wg2x2_conv1x1(const float *X, const float *W, float *Y, int B, int C, int K, int HW, void *stream)
 {
     return wg::conv1x1(X, W, Y, B, C, K, HW, (cudaStream_t)stream);
+}
+
+extern "C" int wg2x2_linear_int8(const void *Q, long long ldq, const float *q_scale, const void *W, long long ldw, const float *w_scale,
+                                 const float *bias, int relu, void *Y, int type, long long ldy, long long B, int HW, int C, int K, int layout,
+                                 void *stream)
+{
+    return wg::linear_int8(Q, ldq, q_scale, W, ldw, w_scale, bias, relu, Y, type, ldy, B, HW, C, K, layout, (cudaStream_t)stream);
 }
 
 extern "C" int wg2x2_stem_prepared_floats(void) { return wg::kStWtFloats; }

@@ -1,0 +1,416 @@
+// Products in 8-bit integers with a scale for each row of either operand (a token or pixel; an output channel):
+//
+//   Y[r][k] = (sum_c q[r][c] w[k][c]) * w_scale[k] * q_scale[r] (+ bias[k])        optionally through a ReLU, in 32 or 16 bits
+//
+// The sums are exact: 32-bit integers in tensor memory (tcgen05 kind::i8), C at most 131071, so 128^2 C < 2^31.  The rest is 32-bit
+// floating point.  Included by conv_tc.cu.
+//
+// Which operand has the 128 lanes of tensor memory goes by the result's layout, so that a warp's store of one column is of consecutive
+// elements: channels last, lanes = output channels (A = the weights, columns = rows of q); NCHW, lanes = pixels (A = q, columns =
+// output channels).  A tile is 128 lanes x N columns; a CTA walks its tiles with two accumulators, so that one is stored while the next
+// is computed.  Where the tiles are too few for the GPU, a cluster of S CTAs shares a tile: each takes a share of the contraction, and
+// the shares (whole numbers, so the order does not matter) meet through distributed shared memory, every CTA finishing N / S columns.
+#pragma once
+
+constexpr int kLiThreads = 320;               // producer, MMA issuer, eight epilogue warps
+constexpr int kLiChunk = 128;                 // bytes of the contraction a stage
+constexpr int kLiMaxStages = 12;
+constexpr int kLiSmem = 232448;               // all that a CTA can have
+constexpr int kLiCtrl = 512 + 8 * 64 * 4;     // barriers; 32 column scales and 32 biases for each epilogue warp
+constexpr int kLiMaxC = 131071;
+
+struct LiParams {
+    void *Y;
+    const float *lane_scale, *col_scale, *bias;     // bias: of the output channels
+    long long ldy;                                  // channels last: elements from row to row
+    int lanes, cols;                                // rows of A and of B
+    int K, HW;                                      // NCHW: channels and pixels of Y's images
+    int N, stages, chunks;                          // columns of a tile; stages of operands; chunks of the contraction
+    int lane_tiles, col_tiles, splits, relu;
+    uint32_t spin_limit;
+    int drop_load;
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+// D[tmem] (+)= A[smem] * B[smem], M=128, K=32, signed 8-bit operands, 32-bit integer accumulator
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Instruction descriptor: D = s32, A = B = s8, both K-major
+__host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N)
+{
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+                   "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+                   "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld8i(uint32_t taddr, int (&r)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+
+// The registers of the loads above pass through the wait, so that nothing that reads them can be moved in front of it
+__device__ __forceinline__ void tmem_wait32(int (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 ::"memory");
+}
+__device__ __forceinline__ void tmem_wait8(int (&r)[8])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) ::"memory");
+}
+
+template <typename T> __device__ __forceinline__ T li_out(float v);
+template <> __device__ __forceinline__ float li_out<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half li_out<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 li_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// (the weights' scale first: of the two it is the one of ordinary size; without a bias the sum is with -0, which changes nothing)
+__device__ __forceinline__ float li_value(int acc, float w_scale, float q_scale, float bias, bool relu)
+{
+    const float v = fmaf(__fmul_rn((float)acc, w_scale), q_scale, bias);
+    return relu ? relu_nan(v) : v;
+}
+
+// 16 lane tiles x all column tiles at a time, so that the CTAs that run together share operands in L2
+__device__ __forceinline__ void li_decode(const LiParams &p, int u, int &lt, int &ct)
+{
+    const int group = u / (16 * p.col_tiles), r = u - group * 16 * p.col_tiles, size = min(16, p.lane_tiles - 16 * group);
+    ct = r / size;
+    lt = 16 * group + r - ct * size;
+}
+
+// What a thread knows about its lane of a tile
+template <bool NCHW, typename T>
+struct LiLane {
+    T *dst;                     // Y at column 0
+    long long step;             // elements from column to column
+    float scale, bias;
+    bool live;
+    __device__ __forceinline__ LiLane(const LiParams &p, int lane_row)
+    {
+        live = lane_row < p.lanes;
+        const int r = live ? lane_row : 0;
+        scale = p.lane_scale[r];
+        bias = !NCHW && p.bias ? p.bias[r] : -0.f;
+        if (NCHW) {
+            const int b = r / p.HW;
+            dst = static_cast<T *>(p.Y) + (long long)b * p.K * p.HW + (r - b * p.HW);
+            step = p.HW;
+        } else {
+            dst = static_cast<T *>(p.Y) + r;
+            step = p.ldy;
+        }
+    }
+};
+
+// Scales (and biases) of 32 columns, in the warp's corner of shared memory
+template <bool NCHW>
+__device__ __forceinline__ void li_stage_columns(const LiParams &p, float *corner, int col0, int lane)
+{
+    const int c = col0 + lane;
+    __syncwarp();
+    corner[lane] = c < p.cols ? p.col_scale[c] : 0.f;
+    if (NCHW) corner[32 + lane] = c < p.cols && p.bias ? p.bias[c] : -0.f;
+    __syncwarp();
+}
+
+// SPLIT: one tile per cluster of `splits` CTAs, else the CTA's tiles in turn
+template <bool NCHW, typename T, bool SPLIT>
+__global__ void __launch_bounds__(kLiThreads, 1)
+linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const LiParams prm)
+{
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t *gen_base = smem_raw + (base - raw);
+    const int stage_bytes = (kBlockM + prm.N) * kLiChunk;
+    const uint32_t ctrl = base + prm.stages * stage_bytes;
+    uint8_t *ctrl_gen = gen_base + prm.stages * stage_bytes;
+    auto full_bar = [&](int s) { return ctrl + 8u * s; };
+    auto empty_bar = [&](int s) { return ctrl + 8u * (kLiMaxStages + s); };
+    auto accf_bar = [&](int b) { return ctrl + 8u * (2 * kLiMaxStages + b); };
+    auto acce_bar = [&](int b) { return ctrl + 8u * (2 * kLiMaxStages + 2 + b); };
+    volatile uint32_t *tmem_ptr_slot = reinterpret_cast<volatile uint32_t *>(ctrl_gen + 8 * (2 * kLiMaxStages + 4));
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(ctrl_gen + 8 * (2 * kLiMaxStages + 5));
+    static_assert(8 * (2 * kLiMaxStages + 6) <= 512, "control block");
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < prm.stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), kEpiWarps); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32((const void *)tmem_ptr_slot), kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (SPLIT) cluster_sync_all();                  // (a CTA's shared memory is written by others only once it runs)
+    tc_fence_after();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_slot, 0);
+    wait_for_previous_kernel(kNumSMs);
+
+    const int rank = SPLIT ? (int)cluster_ctarank() : 0;
+    const int first = SPLIT ? blockIdx.x / prm.splits : blockIdx.x, step = SPLIT ? 1 << 30 : gridDim.x;
+    const int units = prm.lane_tiles * prm.col_tiles;
+    // (at least one chunk for every CTA: splits <= chunks)
+    const int kbeg = SPLIT ? rank * prm.chunks / prm.splits : 0, kend = SPLIT ? (rank + 1) * prm.chunks / prm.splits : prm.chunks;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, loads = 0;
+            uint32_t ph = 0;
+            const uint32_t bytes = (uint32_t)stage_bytes;
+            for (int u = first; u < units && ok; u += step) {
+                int lt, ct;
+                li_decode(prm, u, lt, ct);
+                for (int kc = kbeg; kc < kend; ++kc) {
+                    if (loads++ == prm.drop_load && blockIdx.x == 0) { ok = false; break; }
+                    if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, 0x1C00u | s, prm.spin_limit)) { ok = false; break; }
+                    mbar_expect_tx(full_bar(s), bytes);
+                    const uint32_t dst = base + s * stage_bytes;
+                    tma_load_2d(dst, &mapA, full_bar(s), kc * kLiChunk, lt * kBlockM);
+                    tma_load_2d(dst + kBlockM * kLiChunk, &mapB, full_bar(s), kc * kLiChunk, ct * prm.N);
+                    if (++s == prm.stages) { s = 0; ph ^= 1u; }
+                }
+                if (step == 1 << 30) break;
+            }
+            if (!ok) let_them_land();
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const bool leader = elect_one();
+        const uint32_t idesc = make_idesc_i8(kBlockM, prm.N);
+        int s = 0, buf = 0;
+        uint32_t ph = 0, use = 0;                   // use: rounds of the two accumulators
+        for (int u = first; u < units && ok; u += step) {
+            if (!mbar_wait_warp(acce_bar(buf), (use & 1u) ^ 1u, abort_flag, 0x1D00u | buf, prm.spin_limit)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + (uint32_t)(buf * 256);
+            for (int kc = kbeg; kc < kend; ++kc) {
+                if (!mbar_wait_warp(full_bar(s), ph, abort_flag, 0x1E00u | s, prm.spin_limit)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t at = base + s * stage_bytes;
+                const uint64_t ad = make_desc_k_sw128(at), bd = make_desc_k_sw128(at + kBlockM * kLiChunk);
+                if (leader) {
+#pragma unroll
+                    for (int kk = 0; kk < kLiChunk / 32; ++kk) umma_i8(d_tmem, ad + 2u * kk, bd + 2u * kk, idesc, kc > kbeg || kk > 0 ? 1u : 0u);
+                    umma_commit(empty_bar(s));
+                }
+                __syncwarp();
+                if (++s == prm.stages) { s = 0; ph ^= 1u; }
+            }
+            if (ok && leader) umma_commit(accf_bar(buf));
+            __syncwarp();
+            buf ^= 1;
+            if (buf == 0) ++use;
+            if (step == 1 << 30) break;
+        }
+        if (!ok) let_them_land();
+    } else {
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        float *corner = reinterpret_cast<float *>(ctrl_gen + 512) + (warp - 2) * 64;
+        const uint32_t quarter = (uint32_t)(q * 32) << 16;
+        int buf = 0;
+        uint32_t use = 0;
+        if (!SPLIT) {
+            const int ncols = prm.N >= 64 ? prm.N / 2 : prm.N;          // columns of a warp (N = 32: those of half 0)
+            for (int u = first; u < units; u += step) {
+                int lt, ct;
+                li_decode(prm, u, lt, ct);
+                const LiLane<NCHW, T> me(prm, lt * kBlockM + q * 32 + lane);
+                const int c_first = ct * prm.N + (prm.N >= 64 ? half * ncols : 0);
+                if (!mbar_wait_warp(accf_bar(buf), use & 1u, abort_flag, 0x1F00u | buf, prm.spin_limit)) { ok = false; break; }
+                tc_fence_after();
+                for (int cc = 0; cc < ncols && (prm.N >= 64 || half == 0); cc += 32) {
+                    const int col0 = c_first + cc;
+                    if (col0 >= prm.cols) break;
+                    int r[32];
+                    tmem_ld32(tmem_base + quarter + (uint32_t)(buf * 256 + (prm.N >= 64 ? half * ncols : 0) + cc), r);
+                    li_stage_columns<NCHW>(prm, corner, col0, lane);
+                    tmem_wait32(r);
+                    T *dst = me.dst + col0 * me.step;
+                    const int n = min(min(32, ncols - cc), prm.cols - col0);
+#pragma unroll
+                    for (int x4 = 0; x4 < 8; ++x4) {
+                        float cs[4], cb[4];
+                        *reinterpret_cast<float4 *>(cs) = *reinterpret_cast<const float4 *>(corner + 4 * x4);
+                        if (NCHW) *reinterpret_cast<float4 *>(cb) = *reinterpret_cast<const float4 *>(corner + 32 + 4 * x4);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int x = 4 * x4 + j;
+                            const float v = NCHW ? li_value(r[x], cs[j], me.scale, cb[j], prm.relu) : li_value(r[x], me.scale, cs[j], me.bias, prm.relu);
+                            if (me.live && x < n) dst[x * me.step] = li_out<T>(v);
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acce_bar(buf));
+                buf ^= 1;
+                if (buf == 0) ++use;
+            }
+        } else {
+            // this CTA's share of the sums to the CTAs that finish them: [share][column][lane]
+            ok = mbar_wait_warp(accf_bar(0), 0, abort_flag, 0x1F00u, prm.spin_limit);
+            tc_fence_after();
+            if (ok) {
+                const int mine = prm.N / prm.splits;
+                const uint32_t sums = ctrl + kLiCtrl;
+                for (int c8 = half * 8; c8 < prm.N; c8 += 16) {
+                    int r[8];
+                    tmem_ld8i(tmem_base + quarter + (uint32_t)c8, r);
+                    tmem_wait8(r);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const int c = c8 + x, to = c / mine;
+                        const uint32_t at = mapa_rank(sums + (uint32_t)(((rank * mine + c - to * mine) * kBlockM + q * 32 + lane) * 4), (uint32_t)to);
+                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(r[x]) : "memory");
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    if (SPLIT) {
+        __syncwarp();
+        cluster_sync_all();                         // every thread of every CTA, whatever came before
+        if (warp >= 2) {
+            int lt, ct;
+            li_decode(prm, first, lt, ct);
+            const int q = warp & 3, half = (warp - 2) >> 2, mine = prm.N / prm.splits;
+            const LiLane<NCHW, T> me(prm, lt * kBlockM + q * 32 + lane);
+            const int *sums = reinterpret_cast<const int *>(ctrl_gen + kLiCtrl) + q * 32 + lane;
+            for (int c = half; c < mine; c += 2) {
+                const int col = ct * prm.N + rank * mine + c;
+                if (col >= prm.cols) break;
+                int acc = 0;
+                for (int s = 0; s < prm.splits; ++s) acc += sums[(s * mine + c) * kBlockM];
+                const float cs = prm.col_scale[col], b = NCHW ? (prm.bias ? prm.bias[col] : -0.f) : me.bias;
+                const float v = NCHW ? li_value(acc, cs, me.scale, b, prm.relu) : li_value(acc, me.scale, cs, b, prm.relu);
+                if (me.live) me.dst[col * me.step] = li_out<T>(v);
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+// A (rows, C) tensor of bytes, rows `ld` bytes apart; bytes outside it read as zero
+static bool make_map_codes(CUtensorMap *map, const void *ptr, int C, long long rows, long long ld, int box_rows)
+{
+    EncodeTiledFn fn = encode_fn_raw();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)C, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {(cuuint32_t)kLiChunk, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    auto encode = [&] {
+        return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if ((r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) && cudaFree(nullptr) == cudaSuccess) r = encode();
+    return r == CUDA_SUCCESS;
+}
+
+// Columns of a tile and CTAs that share one, by an estimate in clocks: a chunk of operands comes from L2 at about 64 bytes a clock and
+// SM, a column of 128 lanes is finished in about 10 clocks (beside the next tile's products, where there is one), and a shared tile
+// costs a cluster's barrier and exchange.
+static void li_choose(LiParams &p)
+{
+    double best = 1e300;
+    for (int N = 16; N <= 256; N *= 2) {
+        const long long tiles = (long long)p.lane_tiles * cdiv(p.cols, N);
+        for (int S = 1; S <= 8; S *= 2) {
+            if (S > 1 && (N > 128 || S > p.chunks || tiles * S > kNumSMs)) break;
+            const double chunk = 2.0 * (kBlockM + N), main = (double)cdiv(p.chunks, S) * chunk, store = 10.0 * N / S;
+            const double t = (double)cdivll(tiles * S, kNumSMs) * std::max(main, store) + std::min(main, store) + (S > 1 ? 1000 + 4 * N : 0);
+            if (t < best * 0.999) { best = t; p.N = N; p.splits = S; }
+        }
+    }
+    p.col_tiles = cdiv(p.cols, p.N);
+}
+
+template <bool NCHW, typename T, bool SPLIT>
+static int li_launch(const CUtensorMap &mapA, const CUtensorMap &mapB, const LiParams &p, size_t smem, cudaStream_t st)
+{
+    const long long tiles = (long long)p.lane_tiles * p.col_tiles;
+    if (!SPLIT) return launch(linear_int8_kernel<NCHW, T, false>, dim3((unsigned)std::min<long long>(tiles, kNumSMs)), kLiThreads, smem, st, mapA, mapB, p);
+    return launch_cluster(linear_int8_kernel<NCHW, T, true>, dim3((unsigned)(tiles * p.splits)), p.splits, kLiThreads, smem, st, mapA, mapB, p);
+}
+template <bool NCHW, typename T>
+static int li_launch(const CUtensorMap &mapA, const CUtensorMap &mapB, const LiParams &p, size_t smem, cudaStream_t st)
+{
+    return p.splits > 1 ? li_launch<NCHW, T, true>(mapA, mapB, p, smem, st) : li_launch<NCHW, T, false>(mapA, mapB, p, smem, st);
+}
+
+int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *W, long long ldw, const float *w_scale, const float *bias, int relu,
+                void *Y, int type, long long ldy, long long B, int HW, int C, int K, int layout, cudaStream_t st)
+{
+    if (type < WG2X2_F32 || type > WG2X2_BF16 || (layout != WG2X2_NHWC && layout != WG2X2_NCHW)) return WG2X2_ERR_BAD_ARG;
+    if (B < 0 || HW <= 0 || C <= 0 || K <= 0 || B > 0x7fffffffffffLL / HW) return WG2X2_ERR_BAD_ARG;
+    const long long rows = B * HW;
+    if (!rows) return WG2X2_OK;
+    const bool nchw = layout == WG2X2_NCHW;
+    const int e = type == WG2X2_F32 ? 4 : 2;
+    if (!Q || !q_scale || !W || !w_scale || !Y || ldq < C || ldw < C || (!nchw && ldy < K)) return WG2X2_ERR_BAD_ARG;
+    auto off = [](const void *q, unsigned size) { return (reinterpret_cast<uintptr_t>(q) & (size - 1)) != 0; };
+    if (off(Q, 16) || off(W, 16) || ldq % 16 || ldw % 16 || off(q_scale, 4) || off(w_scale, 4) || off(bias, 4) || off(Y, e)) return WG2X2_ERR_BAD_ARG;
+    if (C > kLiMaxC || rows > 0x7fffffffLL - 256 || K > 0x7fffffff - 256 || ldq >= 1LL << 40 || ldw >= 1LL << 40) return WG2X2_ERR_UNSUPPORTED;
+    const long long ybytes = nchw ? rows * K * e : (long long)K * e, ypitch = nchw ? 0 : ldy * e, ny = nchw ? 1 : rows;
+    auto meets = [&](const void *p, long long ld, long long n, long long count) { return p && rows_overlap(Y, ypitch, ybytes, ny, p, ld, n, count); };
+    if (meets(Q, ldq, C, rows) || meets(W, ldw, C, K) || meets(q_scale, 0, 4 * rows, 1) || meets(w_scale, 0, 4LL * K, 1) || meets(bias, 0, 4LL * K, 1))
+        return WG2X2_ERR_BAD_ARG;
+    LiParams p = {};
+    p.Y = Y; p.ldy = ldy; p.bias = bias; p.K = K; p.HW = HW; p.relu = relu != 0;
+    p.lane_scale = nchw ? q_scale : w_scale;
+    p.col_scale = nchw ? w_scale : q_scale;
+    p.lanes = nchw ? (int)rows : K;
+    p.cols = nchw ? K : (int)rows;
+    p.chunks = cdiv(C, kLiChunk);
+    p.lane_tiles = cdiv(p.lanes, kBlockM);
+    li_choose(p);
+    if ((long long)p.lane_tiles * p.col_tiles > 0x3fffffffLL) return WG2X2_ERR_UNSUPPORTED;
+    const int stage = (kBlockM + p.N) * kLiChunk, other = 1024 + kLiCtrl + (p.splits > 1 ? p.N * kBlockM * 4 : 0);
+    p.stages = std::min({kLiMaxStages, (kLiSmem - other) / stage, std::max(2, p.splits > 1 ? cdiv(p.chunks, p.splits) : kLiMaxStages)});
+    p.spin_limit = wait_limit();
+    p.drop_load = take_drop_load();
+    CUtensorMap mapA, mapB;
+    const void *A = nchw ? Q : W, *Bop = nchw ? W : Q;
+    const long long lda = nchw ? ldq : ldw, ldb = nchw ? ldw : ldq;
+    if (!make_map_codes(&mapA, A, C, p.lanes, lda, kBlockM) || !make_map_codes(&mapB, Bop, C, p.cols, ldb, p.N)) return WG2X2_ERR_LAUNCH;
+    const size_t smem = (size_t)other + (size_t)p.stages * stage;
+    if (type == WG2X2_F32) return nchw ? li_launch<true, float>(mapA, mapB, p, smem, st) : li_launch<false, float>(mapA, mapB, p, smem, st);
+    if (type == WG2X2_F16) return nchw ? li_launch<true, __half>(mapA, mapB, p, smem, st) : li_launch<false, __half>(mapA, mapB, p, smem, st);
+    return nchw ? li_launch<true, __nv_bfloat16>(mapA, mapB, p, smem, st) : li_launch<false, __nv_bfloat16>(mapA, mapB, p, smem, st);
+}

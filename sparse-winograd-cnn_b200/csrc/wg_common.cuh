@@ -7,6 +7,7 @@
 
 #include <initializer_list>
 #include <mutex>
+#include <utility>
 
 #include "../../include/winograd2x2_b200.h"
 
@@ -181,6 +182,17 @@ inline int pair_rows(int B, int C, int nH, int nW, int W, int extra)
     return best ? cdiv(nH, cdiv(nH, best)) : 0;
 }
 
+// Whether two tensors, rows of `na` and `nb` bytes a pitch apart, have bytes in common.  Rows of the same pitch that lie side by side in
+// one buffer do not.
+inline bool rows_overlap(const void *a, long long lda, long long na, long long rows_a, const void *b, long long ldb, long long nb, long long rows_b)
+{
+    const long long x = (long long)reinterpret_cast<uintptr_t>(a), y = (long long)reinterpret_cast<uintptr_t>(b);
+    if (x + (rows_a - 1) * lda + na <= y || y + (rows_b - 1) * ldb + nb <= x) return false;
+    if (lda != ldb || lda <= 0) return true;
+    const long long d = ((y - x) % lda + lda) % lda;          // b's rows behind a's, within the pitch
+    return !(d >= na && d + nb <= lda);
+}
+
 inline int launch_status()
 {
     return cudaGetLastError() == cudaSuccess ? WG2X2_OK : WG2X2_ERR_LAUNCH;
@@ -233,8 +245,9 @@ inline bool grant_smem(const void *kernel, size_t bytes)
     return true;
 }
 
+// `cluster`: CTAs of a cluster along x, for kernels whose cluster has no size of its own
 template <typename... KernelArgs, typename... Args>
-int launch(void (*kernel)(KernelArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args &&...args)
+int launch_cluster(void (*kernel)(KernelArgs...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t st, Args &&...args)
 {
     if (smem > 48 * 1024 && !grant_smem(reinterpret_cast<const void *>(kernel), smem)) return WG2X2_ERR_LAUNCH;
     static const bool pdl_env = [] { const char *e = getenv("WG2X2_PDL"); return !(e && e[0] == '0'); }();
@@ -245,12 +258,25 @@ int launch(void (*kernel)(KernelArgs...), dim3 grid, int threads, size_t smem, c
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = pdl_env && capturing == cudaStreamCaptureStatusNone ? 1 : 0;
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (pdl_env && capturing == cudaStreamCaptureStatusNone) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KernelArgs>(args)...) == cudaSuccess ? launch_status() : WG2X2_ERR_LAUNCH;
+}
+template <typename... KernelArgs, typename... Args>
+int launch(void (*kernel)(KernelArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args &&...args)
+{
+    return launch_cluster(kernel, grid, 1, threads, smem, st, std::forward<Args>(args)...);
 }
 
 }  // namespace wg

@@ -28,7 +28,7 @@ if not os.path.exists(LIB_PATH):
 
 lib = ctypes.CDLL(LIB_PATH)
 
-_p, _i, _z = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_p, _i, _z, _l = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong
 _SIGS = {
     "wg2x2_status_string": (ctypes.c_char_p, [_i]),
     "wg2x2_abi_version": (_i, []),
@@ -60,6 +60,9 @@ _SIGS = {
     "wg2x2_layer_fwd_prepared_scratch": (None, [_i, _i, _i, _i, _i, _i, _i, ctypes.POINTER(_z), ctypes.POINTER(_z)]),
     "wg2x2_conv1x1": (_i, [_p, _p, _p, _i, _i, _i, _i, _p]),
     "wg2x2_conv1x1_preferred": (_i, [_i, _i, _i, _i]),
+    "wg2x2_quantize_int8": (_i, [_p, _i, _l, _p, _l, _p, _l, _i, _i, _i, _i, _p]),
+    "wg2x2_rms_norm_int8": (_i, [_p, _l, _p, _l, _p, _l, _p, _i, ctypes.c_float, _i, _p, _l, _p, _l, _i, _i, _i, _p]),
+    "wg2x2_linear_int8": (_i, [_p, _l, _p, _p, _l, _p, _p, _i, _p, _i, _l, _l, _i, _i, _i, _i, _p]),
     "wg2x2_relu_mean": (_i, [_p, _p, ctypes.c_longlong, _i, _p]),
     "wg2x2_layer_fwd_fused": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p]),
     "wg2x2_layer_fwd_fused_affine": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p]),

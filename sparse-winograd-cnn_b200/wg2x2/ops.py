@@ -176,6 +176,29 @@ def round_tf32(t):
     return torch.where(t.isnan(), t.new_tensor(float("nan")), ((t.view(torch.int32) + 0x1000) & ~0x1FFF).view(torch.float32))
 
 
+def quantize_int8(x, relu=False, layout="NHWC", out=None, scale_out=None):
+    """Codes and scales of the rows of x (float32, float16 or bfloat16), the operands of linear_int8: (q, scale) with q in -127 .. 127
+    and scale = max |x| / 127 of a row, q = x / scale to the nearest whole number (ties to even).  layout="NHWC": x (..., C), rows of a
+    common pitch, q (..., C), scale (...); "NCHW": x (B,C,H,W), q (B,H,W,C), scale (B,H,W).  relu: of relu(x).  The weights (K,C) of a
+    product go through the same call.  Rows of zeros (or with nothing above 2^-119) have scale 0, rows with NaN or infinity scale NaN.
+    q's rows begin on 16-byte boundaries, so for C off a multiple of 16 it is not contiguous."""
+    return _native.quantize_int8(x, relu, _LAYOUTS[layout], out, scale_out)
+
+
+def rms_norm_int8(x, weight, residual=None, eps=1e-6, layout="NHWC", out=None, scale_out=None, residual_out=None):
+    """quantize_int8 of h / sqrt(mean(h^2) + eps) * weight over the channels: (q, scale), or with a residual (q, scale, h), where
+    h = x + residual in x's type, in a tensor of its own or in residual_out (which may be x or residual).  weight (C,): float32 or
+    x's type.  eps at least 1e-30."""
+    return _native.rms_norm_int8(x, weight, residual, eps, _LAYOUTS[layout], out, scale_out, residual_out)
+
+
+def linear_int8(q, scale, w, w_scale, bias=None, relu=False, layout="NHWC", dtype=torch.float32, out=None):
+    """(q @ w.T) * scale * w_scale + bias, optionally through a ReLU: q (..., C) and w (K,C) codes with a scale a row (quantize_int8,
+    rms_norm_int8), sums exact, the result in `dtype` (float32, float16 or bfloat16).  layout="NHWC": (..., K); "NCHW": q (B,H,W,C) ->
+    (B,K,H,W).  bias (K,) float32.  Codes whose rows are not on 16-byte boundaries are copied to such rows first.  C at most 131071."""
+    return _native.linear_int8(q, scale, w, w_scale, bias, relu, _LAYOUTS[layout], dtype, out)
+
+
 def relu_mean(x):
     """x (B,C,H,W) -> (B,C): the mean of relu(x) over the pixels."""
     return _native.relu_mean(x)
