@@ -258,9 +258,9 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
                     const int n = min(min(32, ncols - cc), prm.cols - col0);
 #pragma unroll
                     for (int x4 = 0; x4 < 8; ++x4) {
-                        float cs[4], cb[4];
-                        *reinterpret_cast<float4 *>(cs) = *reinterpret_cast<const float4 *>(corner + 4 * x4);
-                        if (NCHW) *reinterpret_cast<float4 *>(cb) = *reinterpret_cast<const float4 *>(corner + 32 + 4 * x4);
+                        const float4 cs4 = *reinterpret_cast<const float4 *>(corner + 4 * x4);
+                        const float4 cb4 = NCHW ? *reinterpret_cast<const float4 *>(corner + 32 + 4 * x4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float cs[4] = {cs4.x, cs4.y, cs4.z, cs4.w}, cb[4] = {cb4.x, cb4.y, cb4.z, cb4.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int x = 4 * x4 + j;

@@ -7,7 +7,7 @@
 //
 // The norm is a factor of the whole row, so the codes do not depend on it: only the scale does, and codes come out the same whatever
 // the order in which the squares were added.  h is rounded to x's type before anything else looks at it, so that the norm is that of
-// the tensor that is handed on; u is held in 32 bits; the quotient 127 u / a is rounded as in exact arithmetic (code_word).  A row
+// the tensor that is handed on; u is held in 32 bits; the quotient 127 u / a is rounded as in exact arithmetic (code_words).  A row
 // whose a is below 2^-119, where a / 127 leaves the normal numbers, has scale 0 and codes 0.  A row with a NaN or an infinity (or one
 // whose u is beyond 32 bits) has scale NaN and codes 0, so that it stays NaN through a product.
 //
@@ -17,13 +17,14 @@
 
 #include <algorithm>
 
+
 #include "wg_common.cuh"
 
 namespace wg {
 
 constexpr float kTinyRow = 0x1p-119f;
-constexpr float kRound = 12582912.f;        // 1.5 * 2^23: adding it leaves the nearest whole number (ties to even) in the low bits
-constexpr float kNearTie = 0.49998f;        // see code_word
+constexpr float kRound = 12582912.f;        // 1.5 * 2^23: a sum with it is rounded to a whole number (ties to even), in its low bits
+constexpr float kNearTie = 0.49999f;        // see code_words
 
 enum { kQuantize = 0, kNorm = 1, kNormRes = 2 };
 
@@ -35,8 +36,9 @@ struct RowsParams {
     float *scale;
     long long ldx, ldr, ldh, ldq, rows;
     int C, HW;                  // HW: pixels of a plane (NCHW)
-    int group;                  // threads of a row, where a block has several rows
+    int group;                  // threads of a row, where a block has several rows; NCHW: warps of 32 pixels
     int w_f32, relu;
+    unsigned inv;               // NCHW: ceil(2^32 / pieces of a row of codes), see there
     float eps;
 };
 
@@ -49,31 +51,128 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 16 bytes as values
-template <typename T> struct alignas(16) Pack { T v[16 / sizeof(T)]; };
-
-// (plain loads: H may lie over the tensor that is read, which the read-only path must not be used for)
-template <typename T, int N>
-__device__ __forceinline__ Pack<T> load_pack(const T *p, int c0, int C)
+// max(a, |b|) for a that is not negative; NaN stays
+__device__ __forceinline__ float mag_max(float a, float b)
 {
-    Pack<T> r;
-    if (c0 >= 0 && c0 + N <= C) {
-        *reinterpret_cast<uint4 *>(&r) = *reinterpret_cast<const uint4 *>(p + c0);
-    } else {                                            // the ends of a row that does not begin or end on 16 bytes
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+// max(x, low), low = 0 for a ReLU (NaN stays) and -infinity for none
+__device__ __forceinline__ float at_least(float x, float low)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(low));
+    return r;
+}
+
+// 16 bytes, and the N = 4 or 8 values that they are.  Sums are rounded once to the type: the same as through 32 bits, which hold 2 p + 2
+// bits of both types' p.
+struct Pack { unsigned w[4]; };
+__device__ __forceinline__ Pack pack_at(const void *p)
+{
+    const uint4 v = *static_cast<const uint4 *>(p);
+    return Pack{{v.x, v.y, v.z, v.w}};
+}
+template <typename T> struct Types;
+template <> struct Types<float> {
+    static __device__ __forceinline__ void open(const Pack &k, float (&f)[4])
+    {
 #pragma unroll
-        for (int j = 0; j < N; ++j) r.v[j] = c0 + j >= 0 && c0 + j < C ? p[c0 + j] : from_f<T>(0.f);
+        for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(k.w[j]);
+    }
+    static __device__ __forceinline__ Pack sum(const Pack &a, const Pack &b)
+    {
+        Pack k;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k.w[j] = __float_as_uint(__fadd_rn(__uint_as_float(a.w[j]), __uint_as_float(b.w[j])));
+        return k;
+    }
+    static __device__ __forceinline__ unsigned bits(float v) { return __float_as_uint(v); }
+    static __device__ __forceinline__ float value(unsigned b) { return __uint_as_float(b); }
+};
+template <> struct Types<__half> {
+    static __device__ __forceinline__ void open(const Pack &k, float (&f)[8])
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __half2float(__ushort_as_half((unsigned short)(k.w[j >> 1] >> (16 * (j & 1)))));
+    }
+    static __device__ __forceinline__ Pack sum(const Pack &a, const Pack &b)
+    {
+        Pack k;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(k.w[j]) : "r"(a.w[j]), "r"(b.w[j]));
+        return k;
+    }
+    static __device__ __forceinline__ unsigned bits(__half v) { return __half_as_ushort(v); }
+    static __device__ __forceinline__ __half value(unsigned b) { return __ushort_as_half((unsigned short)b); }
+};
+template <> struct Types<__nv_bfloat16> {
+    static __device__ __forceinline__ void open(const Pack &k, float (&f)[8])
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(j & 1 ? k.w[j >> 1] & 0xffff0000u : k.w[j >> 1] << 16);
+    }
+    static __device__ __forceinline__ Pack sum(const Pack &a, const Pack &b)
+    {
+        Pack k;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(k.w[j]) : "r"(a.w[j]), "r"(b.w[j]));
+        return k;
+    }
+    static __device__ __forceinline__ unsigned bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+    static __device__ __forceinline__ __nv_bfloat16 value(unsigned b) { return __ushort_as_bfloat16((unsigned short)b); }
+};
+
+// The values c0 .. c0 + N - 1 of a row of C.  (Plain loads: H may lie over the tensor that is read, which the read-only path must not be
+// used for.)  ODD: a row need not begin or end on 16 bytes, p + c0 does; a piece that reaches beyond the row is read whole where it lies
+// within the tensor [lo, hi), else value by value.
+template <typename T, int N, bool ODD>
+__device__ __forceinline__ Pack load_pack(const T *p, int c0, int C, const T *lo, const T *hi)
+{
+    Pack r = {{0, 0, 0, 0}};
+    if (c0 < C) {
+        if (!ODD || (p + c0 >= lo && p + c0 + N <= hi)) {
+            r = pack_at(p + c0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (c0 + j >= 0 && c0 + j < C) r.w[j * 4 / N] |= Types<T>::bits(p[c0 + j]) << (N == 8 ? 16 * (j & 1) : 0);
+        }
     }
     return r;
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_pack(T *p, int c0, int C, const Pack<T> &r)
+// The same on its way to shared memory (dst, and `at`, its address there), for the thread that asks for it; nothing for c0 >= C
+template <typename T, int N, bool ODD>
+__device__ __forceinline__ void fetch_pack(uint4 *dst, uint32_t at, const T *p, int c0, int C, const T *lo, const T *hi)
 {
-    if (c0 >= 0 && c0 + N <= C) {
-        *reinterpret_cast<uint4 *>(p + c0) = *reinterpret_cast<const uint4 *>(&r);
+    if (c0 >= C) return;
+    if (!ODD || (p + c0 >= lo && p + c0 + N <= hi)) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(p + c0) : "memory");
     } else {
+        const Pack r = load_pack<T, N, ODD>(p, c0, C, lo, hi);
+        *dst = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    }
+}
+// What a piece has of its neighbours' values becomes zero
+template <typename T, int N>
+__device__ __forceinline__ void clear_outside(Pack &r, int c0, int C)
+{
+    if (c0 < 0 || c0 + N > C) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (c0 + j >= 0 && c0 + j < C) p[c0 + j] = r.v[j];
+            if (c0 + j < 0 || c0 + j >= C) r.w[j * 4 / N] &= N == 8 ? (j & 1 ? 0x0000ffffu : 0xffff0000u) : 0u;
+    }
+}
+template <typename T, int N, bool ODD>
+__device__ __forceinline__ void store_pack(T *p, int c0, int C, const Pack &r)
+{
+    if ((!ODD || c0 >= 0) && c0 + N <= C) {
+        *reinterpret_cast<uint4 *>(p + c0) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    } else if (ODD) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (c0 + j >= 0 && c0 + j < C) p[c0 + j] = Types<T>::value(r.w[j * 4 / N] >> (N == 8 ? 16 * (j & 1) : 0));
     }
 }
 __device__ __forceinline__ float weight_at(const RowsParams &p, const float *, int c) { return static_cast<const float *>(p.Wt)[c]; }
@@ -91,12 +190,12 @@ __device__ __forceinline__ void load_weights(const RowsParams &p, int c0, float 
     if (c0 >= 0 && c0 + N <= p.C && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
         if (f32) {
 #pragma unroll
-            for (int j = 0; j < N; j += 4) *reinterpret_cast<float4 *>(w + j) = reinterpret_cast<const float4 *>(at)[j / 4];
+            for (int j = 0; j < N; j += 4) {
+                const float4 t = reinterpret_cast<const float4 *>(at)[j / 4];
+                w[j] = t.x; w[j + 1] = t.y; w[j + 2] = t.z; w[j + 3] = t.w;
+            }
         } else {
-            Pack<T> r;
-            *reinterpret_cast<uint4 *>(&r) = *reinterpret_cast<const uint4 *>(at);
-#pragma unroll
-            for (int j = 0; j < N; ++j) w[j] = to_f(r.v[j]);
+            Types<T>::open(pack_at(at), w);
         }
     } else {
 #pragma unroll
@@ -106,200 +205,306 @@ __device__ __forceinline__ void load_weights(const RowsParams &p, int c0, float 
 
 __device__ __noinline__ unsigned exact_code(float u, float a) { return (unsigned)__double2int_rn((double)u * 127.0 / (double)a); }
 
-// Four codes as a word.  inv = 127 / a rounded, t = u inv rounded: |t - 127 u / a| < 127 * 2^-23 * 1.01 = 1.53e-5, so wherever t is
-// further than 2e-5 from half way between two whole numbers its nearest is that of 127 u / a.  Elsewhere (u = a / 2 is common in
-// 16-bit types) the quotient is taken in 64 bits: 127 u is exact there, and a quotient that is not half way differs from it by more
-// than 2^-33.  a below kTinyRow or not finite: inv = 0, and the caller clears the codes.
-__device__ __forceinline__ unsigned code_word(const float *u, float inv, float a)
+// Codes of N values, four a word.  inv = 127 / a rounded, so |u inv - 127 u / a| <= 127 * 2^-24 = 7.6e-6.  m holds the whole number
+// nearest to u inv, which the fused multiply-add rounds once; d, its distance, is exact to 3e-8.  Wherever |d| <= 0.49999 that number is
+// also the one nearest to 127 u / a.  Elsewhere (u = a / 2 is common in 16-bit types) the quotient is taken in 64 bits: 127 u is exact
+// there, and a quotient that is not half way differs from it by more than 2^-33.  a below kTinyRow or not finite: inv = 0, and the
+// caller clears the codes.
+template <int N>
+__device__ __forceinline__ void code_words(const float (&u)[N], float inv, float a, unsigned (&w)[N / 4])
 {
-    unsigned r[4];
     float off = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float t = __fmul_rn(u[j], inv), m = __fadd_rn(t, kRound);
-        off = fmaxf(off, fabsf(__fsub_rn(t, __fsub_rn(m, kRound))));
-        r[j] = __float_as_uint(m);
+    for (int g = 0; g < N / 4; ++g) {
+        unsigned r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = u[4 * g + j], m = fmaf(x, inv, kRound);
+            off = fmaxf(off, fabsf(fmaf(x, inv, -__fsub_rn(m, kRound))));
+            r[j] = __float_as_uint(m);
+        }
+        w[g] = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
     }
     if (off > kNearTie) {
+#pragma unroll
+        for (int g = 0; g < N / 4; ++g) {
+            unsigned c = 0;
 #pragma unroll 1
-        for (int j = 0; j < 4; ++j) r[j] = exact_code(j == 0 ? u[0] : j == 1 ? u[1] : j == 2 ? u[2] : u[3], a);
+            for (int j = 0; j < 4; ++j)
+                c |= (exact_code(j == 0 ? u[4 * g] : j == 1 ? u[4 * g + 1] : j == 2 ? u[4 * g + 2] : u[4 * g + 3], a) & 0xffu) << (8 * j);
+            w[g] = c;
+        }
     }
-    return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
 }
 
-// A row's largest magnitude, as the bits of |u|: NaN above infinity above everything else
-__device__ __forceinline__ unsigned mag(float u) { return __float_as_uint(u) & 0x7fffffffu; }
-
 struct RowCodes {
-    float inv, a, scale;
+    float inv, a;
     unsigned live;                // all ones, or zero where the codes are 0 whatever u
 };
 constexpr float kDown = 0x1p-100f;     // for a row whose squares leave 32 bits: some |h| is above 2^64 / sqrt(C), all are below 2^128
-__device__ __forceinline__ RowCodes row_codes(unsigned amax)
+__device__ __forceinline__ RowCodes row_codes(float a)
 {
     RowCodes k;
-    k.a = __uint_as_float(amax);
-    const bool ok = k.a >= kTinyRow && amax < 0x7f800000u;
+    k.a = a;
+    const bool ok = a >= kTinyRow && a <= 3.402823466e38f;
     k.live = ok ? 0xffffffffu : 0u;
-    k.inv = ok ? __fdiv_rn(127.f, k.a) : 0.f;
-    k.scale = ok ? __fdiv_rn(k.a, 127.f) : (k.a < kTinyRow ? 0.f : __uint_as_float(0x7fffffffu));
+    k.inv = ok ? __fdiv_rn(127.f, a) : 0.f;
     return k;
 }
-// scale / sqrt(mean square + eps); ss: the sum of the squares of h, or of kDown * h (where eps counts for nothing)
-__device__ __forceinline__ float norm_scale(float scale, float ss, int C, float eps, bool down)
+__device__ __forceinline__ float row_scale(const RowCodes &k)
 {
+    return k.live ? __fdiv_rn(k.a, 127.f) : (k.a < kTinyRow ? 0.f : __uint_as_float(0x7fffffffu));
+}
+// scale / sqrt(mean square + eps); ss: the sum of the squares of h, or of kDown * h (where eps counts for nothing)
+__device__ __forceinline__ float norm_scale(const RowCodes &k, float ss, int C, float eps, bool down)
+{
+    const float scale = row_scale(k);
+    if (!k.live) return scale;
     const float mean = __fdiv_rn(ss, (float)C);
     if (down) return scale > 1.f ? __fdiv_rn(scale * kDown, __fsqrt_rn(mean)) : __fdiv_rn(scale, __fsqrt_rn(mean)) * kDown;
     return __fdiv_rn(scale, __fsqrt_rn(mean + eps));
 }
 
-__device__ __forceinline__ void reduce_group(unsigned &amax, float &ss, int width)
+// The largest magnitude and the sum over `width` lanes (8, 16 or 32)
+template <bool SUM>
+__device__ __forceinline__ void reduce_lanes(float &a, float &ss, int width)
 {
-    for (int o = width >> 1; o; o >>= 1) {
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    }
+    for (int o = width >> 1; o; o >>= 1) a = mag_max(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if (SUM)
+        for (int o = width >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
 }
-// Over the block; every thread has the result, in the same order of additions
-__device__ __forceinline__ void reduce_block(unsigned &amax, float &ss, uint2 *part)
+// Over the block; every thread has the result, from the same order of additions.  `part`: 32 of them, not those of the call before (whose
+// values other warps may still be reading).
+template <bool SUM>
+__device__ __forceinline__ void reduce_block(float &a, float &ss, float2 *part)
 {
-    reduce_group(amax, ss, 32);
-    const int warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_uint2(amax, __float_as_uint(ss));
+    reduce_lanes<SUM>(a, ss, 32);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) part[threadIdx.x >> 5] = make_float2(a, ss);
     __syncthreads();
-    amax = 0;
-    ss = 0.f;
-    for (int w = 0; w < warps; ++w) {
-        const uint2 v = part[w];
-        amax = max(amax, v.x);
-        ss += __uint_as_float(v.y);
+    a = ss = 0.f;
+    if (warps <= 8) {
+        for (int w = 0; w < warps; ++w) {
+            const float2 v = part[w];
+            a = mag_max(a, v.x);
+            ss += v.y;
+        }
+    } else {
+        if (lane < warps) { a = part[lane].x; ss = part[lane].y; }
+        reduce_lanes<SUM>(a, ss, 32);
     }
-    __syncthreads();          // (part may be used again)
 }
 
-// Rows in registers: V loads of 16 bytes a thread.  BLOCK: a row per block, else blockDim.x / group rows.  ODD: rows that do not begin
-// on 16 bytes, or whose length is not a multiple; x, shortcut and sum have the same offset to a 16-byte boundary in every row.  Loads
-// are then of the aligned pieces that a row touches (its ends value by value), and codes reach their own 4 or 8 bytes by a shift with
-// the next lane's.
-template <typename T, int MODE, int V, bool BLOCK, bool ODD>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) rows_kernel(const RowsParams p)
+// Rows in registers: V loads of 16 bytes a thread and tensor.  BLOCK: a row per block, else blockDim.x / group rows.  A warp has
+// neighbouring pieces of a row, V times 32 of them (or of 8 or 16 lanes).
+// AHEAD: a block has several rows (or blocks of rows) in turn, and the loads of the next AHEAD of them are on their way to shared memory
+// while it works on one.  Every thread fetches the pieces that it uses itself, so nothing waits for other threads.
+// ODD: rows that do not begin on 16 bytes, or whose length is not a multiple; x, shortcut and sum have the same offset to a 16-byte
+// boundary in every row.  Loads are then of the aligned pieces that a row touches, and codes reach their own 4 or 8 bytes by a shift
+// with the next lane's.
+template <typename T, int MODE, int V, bool BLOCK, bool ODD, int AHEAD>
+__global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kernel(const RowsParams p)
 {
-    constexpr int N = 16 / sizeof(T), WORDS = N / 4;
-    __shared__ uint2 part[BLOCK ? 32 : 1];
+    constexpr int N = 16 / sizeof(T), WORDS = N / 4, PIECES = MODE == kNormRes ? 2 * V : V, STAGES = AHEAD + 1;
+    constexpr bool SUM = MODE != kQuantize;
+    extern __shared__ uint4 ring[];                     // [STAGES][PIECES][thread], then the weights of the thread's pieces
+    __shared__ float2 part[BLOCK ? 3 * 32 : 1];
+    constexpr bool W_AT_HAND = SUM && AHEAD && !ODD;    // (ODD: which channels a piece has depends on the row)
     wait_for_previous_kernel(kNumSMs);
     const int lane = threadIdx.x & 31;
-    const long long row = BLOCK ? (long long)blockIdx.x : (long long)blockIdx.x * (blockDim.x / p.group) + threadIdx.x / p.group;
-    const int i0 = BLOCK ? threadIdx.x : threadIdx.x & (p.group - 1), step = BLOCK ? blockDim.x : p.group;
-    const bool have = BLOCK || row < p.rows;
-    const int C = have ? p.C : 0;                  // (no element is then loaded or stored)
-    const T *x = static_cast<const T *>(p.X) + (have ? row : 0) * p.ldx;
-    const T *res = MODE == kNormRes ? static_cast<const T *>(p.R) + (have ? row : 0) * p.ldr : nullptr;
-    T *h = MODE == kNormRes ? static_cast<T *>(p.H) + (have ? row : 0) * p.ldh : nullptr;
-    const int mis = ODD ? (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T)) : 0;
+    const int width = BLOCK ? 32 : p.group, at = lane & (width - 1);
+    const int i0 = BLOCK ? (threadIdx.x >> 5) * (32 * V) + lane : at;           // the thread's pieces: i0 + v * width
+    const int per_block = BLOCK ? 1 : blockDim.x / p.group, mine = BLOCK ? 0 : threadIdx.x / p.group;
+    const long long stride = (long long)gridDim.x * per_block, first = (long long)blockIdx.x * per_block;
+    const float low = p.relu ? 0.f : __uint_as_float(0xff800000u);
+    const T *X = static_cast<const T *>(p.X), *R = static_cast<const T *>(p.R);
+    const T *x_end = X + (p.rows - 1) * p.ldx + p.C, *r_end = R + (p.rows - 1) * p.ldr + p.C;
+    auto offset = [&](const T *x) { return ODD ? (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T)) : 0; };
 
-    float u[V][N];
-    {
-        Pack<T> a[V], b[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) a[v] = load_pack<T, N>(x, (i0 + v * step) * N - mis, C);
-        if (MODE == kNormRes) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) b[v] = load_pack<T, N>(res, (i0 + v * step) * N - mis, C);
+    // The block's rows first + mine, + stride, ...: tensors at the row in work, and at the one to be fetched
+    const T *x = X + (first + mine) * p.ldx, *r = R + (first + mine) * p.ldr, *xf = x, *rf = r;
+    T *h = static_cast<T *>(p.H) + (first + mine) * p.ldh;
+    signed char *q = p.Q + (first + mine) * p.ldq;
+    const long long x_step = stride * p.ldx, r_step = stride * p.ldr, h_step = stride * p.ldh, q_step = stride * p.ldq;
+    const uint32_t slot = 16u * blockDim.x, mine_at = (uint32_t)__cvta_generic_to_shared(ring) + 16u * threadIdx.x;
+    uint4 *const mine_ring = ring + threadIdx.x;
+    long long next = first;
+    int put = 0, get = 0, turn = 0;
+    auto fetch = [&] {                  // the loads of the block's row `next`, to stage `put`
+        if (next < p.rows && (BLOCK || next + mine < p.rows)) {
+            const int mis = offset(xf), k = put * PIECES;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) a[v].v[j] = from_f<T>(__fadd_rn(to_f(a[v].v[j]), to_f(b[v].v[j])));
-                store_pack<T, N>(h, (i0 + v * step) * N - mis, C, a[v]);
+                const int c0 = (i0 + v * width) * N - mis;
+                fetch_pack<T, N, ODD>(mine_ring + (k + v) * blockDim.x, mine_at + (k + v) * slot, xf, c0, p.C, X, x_end);
+                if (MODE == kNormRes) fetch_pack<T, N, ODD>(mine_ring + (k + V + v) * blockDim.x, mine_at + (k + V + v) * slot, rf, c0, p.C, R, r_end);
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next += stride;
+        xf += x_step;
+        if (MODE == kNormRes) rf += r_step;
+        put = put + 1 < STAGES ? put + 1 : 0;
+    };
+    float4 *const weights = reinterpret_cast<float4 *>(ring + STAGES * PIECES * blockDim.x) + threadIdx.x;
+    if (AHEAD) {
+        for (int s = 0; s < AHEAD; ++s) fetch();
+        if (W_AT_HAND)
 #pragma unroll
-        for (int v = 0; v < V; ++v)
+            for (int v = 0; v < V; ++v) {
+                float w[N];
+                load_weights<T, N>(p, (i0 + v * width) * N, w);
 #pragma unroll
-            for (int j = 0; j < N; ++j) u[v][j] = to_f(a[v].v[j]);
-    }
-    unsigned amax = 0;
-    float ss = 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (MODE != kQuantize) {
-            float w[N];
-            load_weights<T, N>(p, C ? (i0 + v * step) * N - mis : p.C, w);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                ss = fmaf(u[v][j], u[v][j], ss);
-                u[v][j] = __fmul_rn(u[v][j], w[j]);
+                for (int j = 0; j < N; j += 4) weights[(v * N + j) / 4 * blockDim.x] = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
             }
-        } else if (p.relu) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) u[v][j] = relu_nan(u[v][j]);
+    }
+    for (long long base = first; base < p.rows; base += stride) {
+        const long long row = base + mine;
+        const bool have = BLOCK || row < p.rows;
+        const int C = have ? p.C : -N;                  // (nothing of a row that is not there)
+        const int mis = offset(x);
+        float u[V][N];
+        if (AHEAD) {
+            fetch();
+            asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j) amax = max(amax, mag(u[v][j]));
-    }
-    if (BLOCK) reduce_block(amax, ss, part);
-    else reduce_group(amax, ss, p.group);
-    RowCodes k = row_codes(amax);
-    if (MODE != kQuantize) {
-        bool down = k.live && !(ss <= 3.402823466e38f);
-        if (BLOCK ? down : __any_sync(0xffffffffu, down)) {        // the squares of a row of large values: once more, scaled (h as it was stored)
-            float s2 = 0.f;
-            unsigned none = 0;
-#pragma unroll 1
-            for (int v = 0; v < V; ++v)
-                for (int j = 0; j < N; ++j) {
-                    const int c = (i0 + v * step) * N - mis + j;
-                    if (c < 0 || c >= C) continue;
-                    const float f = to_f(MODE == kNormRes ? h[c] : x[c]) * kDown;
-                    s2 = fmaf(f, f, s2);
+        for (int v = 0; v < V; ++v) {
+            const int c0 = (i0 + v * width) * N - mis;
+            Pack a = {{0, 0, 0, 0}}, b = a;
+            if (AHEAD) {
+                if (c0 < C) {
+                    a = pack_at(mine_ring + (get * PIECES + v) * blockDim.x);
+                    if (MODE == kNormRes) b = pack_at(mine_ring + (get * PIECES + V + v) * blockDim.x);
                 }
-            if (BLOCK) reduce_block(none, s2, part);
-            else reduce_group(none, s2, p.group);
-            if (down) ss = s2;
+            } else {
+                a = load_pack<T, N, ODD>(x, c0, C, X, x_end);
+                if (MODE == kNormRes) b = load_pack<T, N, ODD>(r, c0, C, R, r_end);
+            }
+            if (ODD) clear_outside<T, N>(a, c0, C);
+            if (MODE == kNormRes) {
+                if (ODD) clear_outside<T, N>(b, c0, C);
+                a = Types<T>::sum(a, b);
+                store_pack<T, N, ODD>(h, c0, C, a);
+            }
+            Types<T>::open(a, u[v]);
         }
-        k.scale = k.live ? norm_scale(k.scale, ss, p.C, p.eps, down) : k.scale;
-    }
-    if (have && i0 == 0) p.scale[row] = k.scale;
-
-    signed char *q = p.Q + (have ? row : 0) * p.ldq;
+        get = get + 1 < STAGES ? get + 1 : 0;
+        float amax = 0.f, ss = 0.f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int i = i0 + v * step, c0 = i * N;
-        unsigned w[2 * WORDS];
+        for (int v = 0; v < V; ++v) {
+            if (MODE != kQuantize) {
+                float w[N];
+                if (W_AT_HAND) {
 #pragma unroll
-        for (int g = 0; g < WORDS; ++g) w[g] = code_word(u[v] + 4 * g, k.inv, k.a) & k.live;
-        if (!ODD) {
-            if (c0 < C) {
-                if (WORDS == 2) *reinterpret_cast<uint2 *>(q + c0) = make_uint2(w[0], w[WORDS - 1]);
-                else *reinterpret_cast<unsigned *>(q + c0) = w[0];
-            }
-        } else {
-            // codes of channels c0 - mis .. c0 - mis + N - 1 here, the next N in the next lane (not behind the last lane of a warp or
-            // of a row's group).  A lane with a next one stores channels c0 .. c0 + N - 1, else what it has of them; the first lane also
-            // what lies in front of c0.
+                    for (int j = 0; j < N; j += 4) {
+                        const float4 t = weights[(v * N + j) / 4 * blockDim.x];
+                        w[j] = t.x; w[j + 1] = t.y; w[j + 2] = t.z; w[j + 3] = t.w;
+                    }
+                } else {
+                    load_weights<T, N>(p, (i0 + v * width) * N - mis, w);
+                }
 #pragma unroll
-            for (int g = 0; g < WORDS; ++g) w[WORDS + g] = __shfl_down_sync(0xffffffffu, w[g], 1);
-            const int width = BLOCK ? 32 : p.group, at = BLOCK ? lane : i0;
-            const bool next = at < width - 1;
-            const int own = N - mis, count = min(next ? N : own, C - c0);
-            if (at == 0)
-                for (int j = 0; j < mis; ++j)
-                    if (c0 - mis + j >= 0 && c0 - mis + j < C) q[c0 - mis + j] = (signed char)(w[j >> 2] >> (8 * (j & 3)));
-            unsigned o[WORDS];
-#pragma unroll
-            for (int g = 0; g < WORDS; ++g) {
-                unsigned lo = w[g], hi = w[g + 1];
-                if (WORDS == 2 && (mis & 4)) { lo = hi; hi = w[min(g + 2, 2 * WORDS - 1)]; }
-                o[g] = __funnelshift_r(lo, hi, 8 * (mis & 3));
-            }
-            if (count == N && (reinterpret_cast<uintptr_t>(q) & (N - 1)) == 0) {
-                if (WORDS == 2) *reinterpret_cast<uint2 *>(q + c0) = make_uint2(o[0], o[WORDS - 1]);
-                else *reinterpret_cast<unsigned *>(q + c0) = o[0];
+                for (int j = 0; j < N; ++j) {
+                    ss = fmaf(u[v][j], u[v][j], ss);
+                    u[v][j] = __fmul_rn(u[v][j], w[j]);
+                }
             } else {
 #pragma unroll
+                for (int j = 0; j < N; ++j) u[v][j] = at_least(u[v][j], low);
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) amax = mag_max(amax, u[v][j]);
+        }
+        if (BLOCK) reduce_block<SUM>(amax, ss, part + 32 * turn);
+        else reduce_lanes<SUM>(amax, ss, width);
+        turn ^= 1;
+        RowCodes k = row_codes(amax);
+        if (MODE != kQuantize) {
+            const bool down = k.live && !(ss <= 3.402823466e38f);
+            if (BLOCK ? down : __any_sync(0xffffffffu, down)) {        // the squares of a row of large values: once more, scaled (h as it was stored)
+                float s2 = 0.f, none = 0.f;
+#pragma unroll 1
+                for (int v = 0; v < V; ++v)
+                    for (int j = 0; j < N; ++j) {
+                        const int c = (i0 + v * width) * N - mis + j;
+                        if (c < 0 || c >= C) continue;
+                        const float f = to_f(MODE == kNormRes ? h[c] : x[c]) * kDown;
+                        s2 = fmaf(f, f, s2);
+                    }
+                if (BLOCK) {
+                    reduce_block<true>(none, s2, part + 64);
+                    __syncthreads();
+                } else {
+                    reduce_lanes<true>(none, s2, width);
+                }
+                if (down) ss = s2;
+            }
+            if (have && i0 == 0) p.scale[row] = norm_scale(k, ss, p.C, p.eps, down);
+        } else if (have && i0 == 0) {
+            p.scale[row] = row_scale(k);
+        }
+
+        unsigned w[V][WORDS];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            code_words<N>(u[v], k.inv, k.a, w[v]);
+#pragma unroll
+            for (int g = 0; g < WORDS; ++g) w[v][g] &= k.live;
+        }
+        if (!ODD) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int c0 = (i0 + v * width) * N;
+                if (c0 < C) {
+                    if (WORDS == 2) *reinterpret_cast<uint2 *>(q + c0) = make_uint2(w[v][0], w[v][WORDS - 1]);
+                    else *reinterpret_cast<unsigned *>(q + c0) = w[v][0];
+                }
+            }
+        } else {
+            // Piece i has the codes of channels i N - mis .. i N - mis + N - 1; with the first mis of the next piece, those of i N .. i N + N - 1.
+            // The last piece of a warp's (or group's) has no next one at hand and stores what it has; the first stores what lies in front.
+            const bool whole = (reinterpret_cast<uintptr_t>(q) & (N - 1)) == 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                unsigned s[2 * WORDS + 1];
+#pragma unroll
+                for (int g = 0; g < WORDS; ++g) {
+                    s[g] = w[v][g];
+                    s[WORDS + g] = __shfl_down_sync(0xffffffffu, w[v][g], 1);
+                    if (v + 1 < V) {
+                        const unsigned wrapped = __shfl_sync(0xffffffffu, w[v + 1 < V ? v + 1 : v][g], lane & ~(width - 1));
+                        if (at == width - 1) s[WORDS + g] = wrapped;
+                    }
+                }
+                s[2 * WORDS] = 0;
+                const bool next = v + 1 < V || at < width - 1;
+                const int c0 = (i0 + v * width) * N, count = min(next ? N : N - mis, C - c0);
+                unsigned o[WORDS];
+#pragma unroll
+                for (int g = 0; g < WORDS; ++g) {
+                    const bool far = WORDS == 2 && (mis & 4);
+                    o[g] = __funnelshift_r(far ? s[g + 1] : s[g], far ? s[g + 2] : s[g + 1], 8 * (mis & 3));
+                }
+                if (count == N && whole) {
+                    if (WORDS == 2) *reinterpret_cast<uint2 *>(q + c0) = make_uint2(o[0], o[WORDS - 1]);
+                    else *reinterpret_cast<unsigned *>(q + c0) = o[0];
+                } else if (count > 0) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j)
+                        if (j < count) q[c0 + j] = (signed char)(o[j >> 2] >> (8 * (j & 3)));
+                }
+            }
+            if (BLOCK && i0 > 0 && lane == 0) {
+                const int c0 = i0 * N - mis;
+#pragma unroll
                 for (int j = 0; j < N; ++j)
-                    if (j < count) q[c0 + j] = (signed char)(o[j >> 2] >> (8 * (j & 3)));
+                    if (j < mis && c0 + j < C) q[c0 + j] = (signed char)(w[0][j >> 2] >> (8 * (j & 3)));
             }
         }
+        x += x_step;
+        if (MODE == kNormRes) { r += r_step; h += h_step; }
+        q += q_step;
     }
 }
 
@@ -307,7 +512,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) rows_kernel(const RowsPara
 template <typename T, int MODE>
 __global__ void __launch_bounds__(512) rows_any_kernel(const RowsParams p)
 {
-    __shared__ uint2 part[32];
+    __shared__ float2 part[2 * 32];
     wait_for_previous_kernel(kNumSMs);
     const long long row = blockIdx.x;
     const T *x = static_cast<const T *>(p.X) + row * p.ldx;
@@ -318,149 +523,186 @@ __global__ void __launch_bounds__(512) rows_any_kernel(const RowsParams p)
         const float v = to_f(again[c]);
         return MODE != kQuantize ? __fmul_rn(v, weight_at(p, (const T *)nullptr, c)) : p.relu ? relu_nan(v) : v;
     };
-    unsigned amax = 0;
-    float ss = 0.f;
+    float amax = 0.f, ss = 0.f;
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
         if (MODE == kNormRes) h[c] = from_f<T>(__fadd_rn(to_f(x[c]), to_f(res[c])));
         const float v = to_f(again[c]);
         ss = fmaf(v, v, ss);
-        amax = max(amax, mag(value(c)));
+        amax = mag_max(amax, value(c));
     }
-    reduce_block(amax, ss, part);
+    reduce_block<true>(amax, ss, part);
     RowCodes k = row_codes(amax);
     if (MODE != kQuantize && k.live) {
         const bool down = !(ss <= 3.402823466e38f);
         if (down) {
-            unsigned none = 0;
+            float none = 0.f;
             ss = 0.f;
             for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
                 const float f = to_f(again[c]) * kDown;
                 ss = fmaf(f, f, ss);
             }
-            reduce_block(none, ss, part);
+            reduce_block<true>(none, ss, part + 32);
         }
-        k.scale = norm_scale(k.scale, ss, p.C, p.eps, down);
+        if (threadIdx.x == 0) p.scale[row] = norm_scale(k, ss, p.C, p.eps, down);
+    } else if (threadIdx.x == 0) {
+        p.scale[row] = row_scale(k);
     }
-    if (threadIdx.x == 0) p.scale[row] = k.scale;
     signed char *q = p.Q + row * p.ldq;
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
         const float u[4] = {value(c), 0.f, 0.f, 0.f};
-        q[c] = (signed char)(code_word(u, k.inv, k.a) & k.live);
+        unsigned w[1];
+        code_words<4>(u, k.inv, k.a, w);
+        q[c] = (signed char)(w[0] & k.live);
     }
 }
 
-// NCHW: 32 pixels a block, lane = pixel (of any images), so that a load is 32 consecutive values of a plane; a warp takes four
-// neighbouring channels at a time, whose codes are a word.  NQ: groups of four channels that a thread keeps (0: any number, read a
-// second time).  The words are turned through shared memory and leave as rows.
+// NCHW: lane = pixel (of any images), so that a load is 32 consecutive values of a plane.  p.group warps share a tile of 32 pixels, each
+// with groups of four neighbouring channels, whose codes are a word: NQ groups a thread (0: any number, read a second time).  As many as
+// registers allow, because a thread has costs of its own per pixel (its image, the divisions, the meeting of its warps).  The words are turned through shared memory and leave as pieces of rows.
 template <typename T, int MODE, int NQ>
 __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
 {
-    extern __shared__ unsigned turned[];            // [32][pitch]
-    __shared__ uint2 part[16][32];
+    extern __shared__ unsigned turned_all[];        // [tile of the block][32][pitch]
+    __shared__ float2 part[2][16][32];
+    constexpr bool SUM = MODE != kQuantize;
     wait_for_previous_kernel(kNumSMs);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const long long row0 = (long long)blockIdx.x * 32, row = row0 + lane;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = p.group;
+    const int tile = warp / share, wi = warp - tile * share, tiles = (blockDim.x >> 5) / share;
+    const long long row0 = ((long long)blockIdx.x * tiles + tile) * 32, row = row0 + lane;
     const bool have = row < p.rows;
-    const long long b = have ? row / p.HW : 0, base = b * p.C * p.HW + (have ? row - b * p.HW : 0);
+    long long base = 0;
+    if (have) {
+        if (p.rows <= 0x7fffffffLL) {
+            const unsigned b = (unsigned)row / (unsigned)p.HW;
+            base = (long long)b * p.C * p.HW + ((unsigned)row - b * (unsigned)p.HW);
+        } else {
+            const long long b = row / p.HW;
+            base = b * p.C * p.HW + (row - b * p.HW);
+        }
+    }
     const T *x = static_cast<const T *>(p.X) + base;
     const T *res = MODE == kNormRes ? static_cast<const T *>(p.R) + base : nullptr;
     T *h = MODE == kNormRes ? static_cast<T *>(p.H) + base : nullptr;
-    const int words = (p.C + 3) >> 2, pitch = words | 1;
-    const long long HW = p.HW;
-    auto value = [&](float v, int c) { return MODE != kQuantize ? __fmul_rn(v, weight_at(p, (const T *)nullptr, c)) : p.relu ? relu_nan(v) : v; };
+    const int words = (p.C + 3) >> 2, pitch = words | 1, C = have ? p.C : 0;
+    const unsigned HW = p.HW;                       // (a channel's offset in its image fits 31 bits, but for NQ = 0)
+    const float low = p.relu ? 0.f : __uint_as_float(0xff800000u);
+    auto value = [&](float v, int c) { return MODE != kQuantize ? __fmul_rn(v, weight_at(p, (const T *)nullptr, c)) : at_least(v, low); };
 
     constexpr int KEEP = NQ ? NQ : 1;
     float u[KEEP][4];
-    unsigned amax = 0;
-    float ss = 0.f;
+    float amax = 0.f, ss = 0.f;
     if (NQ) {
 #pragma unroll
         for (int g = 0; g < KEEP; ++g)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int c = 4 * (warp + g * warps) + j;
-                u[g][j] = have && c < p.C ? to_f(x[c * HW]) : 0.f;
+                const unsigned c = 4 * (wi + g * share) + j;
+                u[g][j] = c < (unsigned)C ? to_f(x[c * HW]) : 0.f;
             }
         if (MODE == kNormRes) {
+            constexpr int HALF = KEEP > 8 ? 8 : KEEP;
 #pragma unroll
-            for (int g = 0; g < KEEP; ++g)
+            for (int g0 = 0; g0 < KEEP; g0 += HALF) {
+                float r[HALF][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int c = 4 * (warp + g * warps) + j;
-                    if (!have || c >= p.C) continue;
-                    const T s = from_f<T>(__fadd_rn(u[g][j], to_f(res[c * HW])));
-                    h[c * HW] = s;
-                    u[g][j] = to_f(s);
-                }
+                for (int g = 0; g < HALF; ++g)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const unsigned c = 4 * (wi + (g0 + g) * share) + j;
+                        r[g][j] = c < (unsigned)C ? to_f(res[c * HW]) : 0.f;
+                    }
+#pragma unroll
+                for (int g = 0; g < HALF; ++g)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const unsigned c = 4 * (wi + (g0 + g) * share) + j;
+                        const T s = from_f<T>(__fadd_rn(u[g0 + g][j], r[g][j]));
+                        if (c < (unsigned)C) h[c * HW] = s;
+                        u[g0 + g][j] = to_f(s);
+                    }
+            }
         }
 #pragma unroll
-        for (int g = 0; g < KEEP; ++g)
+        for (int g = 0; g < KEEP; ++g) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int c = 4 * (warp + g * warps) + j;
-                ss = fmaf(u[g][j], u[g][j], ss);
-                u[g][j] = c < p.C ? value(u[g][j], c) : 0.f;
-                amax = max(amax, mag(u[g][j]));
+                const int c = 4 * (wi + g * share) + j;
+                if (SUM) ss = fmaf(u[g][j], u[g][j], ss);
+                u[g][j] = MODE != kQuantize && c >= p.C ? 0.f : value(u[g][j], c);
+                amax = mag_max(amax, u[g][j]);
             }
+        }
     } else {
-        for (int c = warp; have && c < p.C; c += warps) {
-            float v = to_f(x[c * HW]);
+        for (int c = wi; c < C; c += share) {
+            const long long o = (long long)c * HW;
+            float v = to_f(x[o]);
             if (MODE == kNormRes) {
-                const T s = from_f<T>(__fadd_rn(v, to_f(res[c * HW])));
-                h[c * HW] = s;
+                const T s = from_f<T>(__fadd_rn(v, to_f(res[o])));
+                h[o] = s;
                 v = to_f(s);
             }
             ss = fmaf(v, v, ss);
-            amax = max(amax, mag(value(v, c)));
+            amax = mag_max(amax, value(v, c));
         }
     }
-    // a pixel's maximum and sum over the warps; every warp adds in the same order
-    auto over_warps = [&](unsigned &m, float &s) {
-        part[warp][lane] = make_uint2(m, __float_as_uint(s));
+    // a pixel's maximum and sum over the warps that share it; each of them adds in the same order
+    auto over_warps = [&](float &m, float &s, int turn) {
+        if (share == 1) return;
+        part[turn][warp][lane] = make_float2(m, s);
         __syncthreads();
-        m = 0;
-        s = 0.f;
-        for (int w = 0; w < warps; ++w) {
-            const uint2 v = part[w][lane];
-            m = max(m, v.x);
-            s += __uint_as_float(v.y);
+        m = s = 0.f;
+        for (int w = 0; w < share; ++w) {
+            const float2 v = part[turn][tile * share + w][lane];
+            m = mag_max(m, v.x);
+            s += v.y;
         }
-        __syncthreads();
     };
-    over_warps(amax, ss);
+    over_warps(amax, ss, 0);
     RowCodes k = row_codes(amax);
     if (MODE != kQuantize) {
         const bool down = k.live && !(ss <= 3.402823466e38f);
-        if (__any_sync(0xffffffffu, down)) {       // (the same in every warp: all have the same sums)
-            const T *again = MODE == kNormRes ? h : x;
-            float s2 = 0.f;
-            unsigned none = 0;
-            for (int c = warp; have && c < p.C; c += warps) {
-                const float f = to_f(again[c * HW]) * kDown;
+        const bool any = share == 1 ? __any_sync(0xffffffffu, down) : __syncthreads_or(down);
+        if (any) {
+            const T *again = MODE == kNormRes ? h : x;          // (h as any of these warps stored it: there has been a barrier)
+            float s2 = 0.f, none = 0.f;
+            for (int c = wi; c < C; c += share) {
+                const float f = to_f(again[(long long)c * HW]) * kDown;
                 s2 = fmaf(f, f, s2);
             }
-            over_warps(none, s2);
+            over_warps(none, s2, 1);
             if (down) ss = s2;
         }
-        k.scale = k.live ? norm_scale(k.scale, ss, p.C, p.eps, down) : k.scale;
+        if (wi == 0 && have) p.scale[row] = norm_scale(k, ss, p.C, p.eps, down);
+    } else if (wi == 0 && have) {
+        p.scale[row] = row_scale(k);
     }
-    if (warp == 0 && have) p.scale[row] = k.scale;
     if (NQ) {
+        unsigned *turned = turned_all + tile * 32 * pitch;
 #pragma unroll
         for (int g = 0; g < KEEP; ++g) {
-            const int q = warp + g * warps;
-            if (q < words) turned[lane * pitch + q] = code_word(u[g], k.inv, k.a) & k.live;
+            const int q = wi + g * share;
+            unsigned w[1];
+            code_words<4>(u[g], k.inv, k.a, w);
+            if (q < words) turned[lane * pitch + q] = w[0] & k.live;
         }
-        __syncthreads();
-        const int n = (int)min(32LL, p.rows - row0);
-        const bool whole = (p.ldq & 3) == 0 && (reinterpret_cast<uintptr_t>(p.Q) & 3u) == 0;
-        for (int i = threadIdx.x; i < n * words; i += blockDim.x) {
-            const int r = i / words, q = i - r * words;
-            const unsigned w = turned[r * pitch + q];
-            signed char *dst = p.Q + (row0 + r) * p.ldq + 4 * q;
-            if (whole && 4 * q + 4 <= p.C) {
-                *reinterpret_cast<unsigned *>(dst) = w;
+        if (share == 1) __syncwarp();
+        else __syncthreads();
+        const int n = row0 < p.rows ? (int)min(32LL, p.rows - row0) : 0;
+        signed char *rows = p.Q + row0 * p.ldq;
+        const unsigned align = (unsigned)reinterpret_cast<uintptr_t>(p.Q) | (unsigned)p.ldq;
+        // pieces of 16 bytes, else words, the last one of a row byte by byte; i / pieces = the high word of i * inv
+        const bool by16 = p.C % 16 == 0 && (align & 15u) == 0;
+        const int pieces = by16 ? words >> 2 : words;
+        for (int i = 32 * wi + lane; i < n * pieces; i += 32 * share) {
+            const int r = pieces == 1 ? i : (int)__umulhi((unsigned)i, p.inv), q = i - r * pieces;
+            const unsigned *src = turned + r * pitch + (by16 ? 4 * q : q);
+            signed char *dst = rows + r * p.ldq + (by16 ? 16 * q : 4 * q);
+            if (by16) {
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(src[0], src[1], src[2], src[3]);
+            } else if ((align & 3u) == 0 && 4 * q + 4 <= p.C) {
+                *reinterpret_cast<unsigned *>(dst) = *src;
             } else {
+                const unsigned w = *src;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (4 * q + j < p.C) dst[j] = (signed char)(w >> (8 * j));
@@ -468,14 +710,16 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
         }
     } else {
         // (h as any warp stored it: over_warps is a barrier)
-        for (int q = warp; have && q < words; q += warps) {
+        for (int q = wi; 4 * q < C; q += share) {
             float v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int c = 4 * q + j;
-                v[j] = c < p.C ? value(to_f((MODE == kNormRes ? h : x)[c * HW]), c) : 0.f;
+                v[j] = c < p.C ? value(to_f((MODE == kNormRes ? h : x)[(long long)c * HW]), c) : 0.f;
             }
-            const unsigned w = code_word(v, k.inv, k.a) & k.live;
+            unsigned codes[1];
+            code_words<4>(v, k.inv, k.a, codes);
+            const unsigned w = codes[0] & k.live;
             signed char *dst = p.Q + row * p.ldq + 4 * q;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -487,11 +731,27 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
 // ---------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------
-template <typename T, int MODE, int V, bool BLOCK>
-static int launch_rows(bool odd, unsigned blocks, int threads, const RowsParams &p, cudaStream_t st)
+// AHEAD = 0: as many blocks as there are rows (or blocks of rows); else at most as many as run at once
+template <typename T, int MODE, int V, bool BLOCK, bool ODD, int AHEAD>
+static int launch_rows(int threads, const RowsParams &p, cudaStream_t st)
 {
-    return odd ? launch(rows_kernel<T, MODE, V, BLOCK, true>, dim3(blocks), threads, 0, st, p)
-               : launch(rows_kernel<T, MODE, V, BLOCK, false>, dim3(blocks), threads, 0, st, p);
+    auto *kernel = rows_kernel<T, MODE, V, BLOCK, ODD, AHEAD>;
+    const size_t smem = AHEAD ? (size_t)((AHEAD + 1) * (MODE == kNormRes ? 2 * V : V) * 16 + (MODE != kQuantize && !ODD ? V * (16 / (int)sizeof(T)) * 4 : 0)) * threads : 0;
+    long long blocks = cdivll(p.rows, BLOCK ? 1 : threads / p.group);
+    if (AHEAD) {
+        static const int regs = [&] {
+            cudaFuncAttributes a;
+            return cudaFuncGetAttributes(&a, reinterpret_cast<const void *>(kernel)) == cudaSuccess && a.numRegs > 0 ? (a.numRegs + 7) / 8 * 8 : 128;
+        }();
+        const long long at_once = std::max(1, std::min({2048 / threads, 65536 / (regs * threads), (int)(228 * 1024 / (smem + 2048))}));
+        blocks = std::min(blocks, kNumSMs * at_once);
+    }
+    return launch(kernel, dim3((unsigned)blocks), threads, smem, st, p);
+}
+template <typename T, int MODE, int V, bool BLOCK, int AHEAD>
+static int launch_rows(bool odd, int threads, const RowsParams &p, cudaStream_t st)
+{
+    return odd ? launch_rows<T, MODE, V, BLOCK, true, AHEAD>(threads, p, st) : launch_rows<T, MODE, V, BLOCK, false, AHEAD>(threads, p, st);
 }
 
 template <typename T, int MODE>
@@ -505,36 +765,52 @@ static int rows_int8(RowsParams p, cudaStream_t st)
     const bool odd = ox || p.C % N || p.ldq % N || (reinterpret_cast<uintptr_t>(p.Q) & (N - 1));
     const long long nv = odd ? cdivll((long long)p.C + N - 1, N) : p.C / N;
     if (!same || nv > 4096) return launch(rows_any_kernel<T, MODE>, dim3((unsigned)p.rows), 512, 0, st, p);
-    // A few rows: as many threads a row as it has loads.  Many: a row in a warp or a part of one up to 128 loads.
+    // A few rows: as many threads a row as it has loads.  Many: a row in a warp or a part of one up to 128 loads, else four or eight loads a
+    // thread.
     const bool few = p.rows < 2 * kNumSMs;
-    if (nv <= 32 || (nv <= 128 && !few)) {
+    if (few && nv > 32 && nv <= 1024) return launch_rows<T, MODE, 1, true, 0>(odd, (int)(cdivll(nv, 32) * 32), p, st);
+    if (nv <= 128) {
+        const bool little = p.rows * nv < 8 * 256 * kNumSMs;       // less than a round of blocks of four loads a thread
+        const int V = little ? 1 : nv >= 8 ? 4 : nv >= 4 ? 2 : 1;
+        for (p.group = 2; p.group < 32 && p.group * V < nv;) p.group *= 2;
+        if (p.group * V >= nv) {
+            if (little) return launch_rows<T, MODE, 1, false, 0>(odd, 256, p, st);
+            if (V == 1) return launch_rows<T, MODE, 1, false, 3>(odd, 256, p, st);
+            if (V == 2) return launch_rows<T, MODE, 2, false, 2>(odd, 256, p, st);
+        }
         p.group = 32;
-        while (p.group > 8 && p.group / 2 >= nv) p.group /= 2;
-        const unsigned blocks = (unsigned)cdivll(p.rows, 256 / p.group);
-        if (nv <= 32) return launch_rows<T, MODE, 1, false>(odd, blocks, 256, p, st);
-        if (nv <= 64) return launch_rows<T, MODE, 2, false>(odd, blocks, 256, p, st);
-        return launch_rows<T, MODE, 4, false>(odd, blocks, 256, p, st);
+        while (p.group > 2 && p.group * 2 >= nv) p.group /= 2;
+        return launch_rows<T, MODE, 4, false, 1>(odd, 256, p, st);
     }
-    const int V = few && nv <= 1024 ? 1 : nv <= 2048 ? 2 : 4;
-    const int threads = (int)(cdivll(cdivll(nv, V), 32) * 32);
-    if (V == 1) return launch_rows<T, MODE, 1, true>(odd, (unsigned)p.rows, threads, p, st);
-    if (V == 2) return launch_rows<T, MODE, 2, true>(odd, (unsigned)p.rows, threads, p, st);
-    return launch_rows<T, MODE, 4, true>(odd, (unsigned)p.rows, threads, p, st);
+    if (nv <= 2048) return launch_rows<T, MODE, 4, true, 1>(odd, (int)(cdivll(nv, 128) * 32), p, st);
+    return launch_rows<T, MODE, 8, true, 0>(odd, (int)(cdivll(nv, 256) * 32), p, st);
 }
 
 template <typename T, int MODE>
-static int nchw_int8(const RowsParams &p, cudaStream_t st)
+static int nchw_int8(RowsParams p, cudaStream_t st)
 {
-    const long long blocks = cdivll(p.rows, 32);
+    const int words = cdiv(p.C, 4); const int most = words <= 128 ? 8 : 16;
+    const long long tiles = cdivll(p.rows, 32);
+    // warps that share 32 pixels: as few as the registers allow, more where the pixels are few
+    int share = 1;
+    while (share < 16 && words > share * most) share *= 2;
+    while (share < 16 && words >= 4 * share && tiles * share < 8 * kNumSMs) share *= 2;
+    const bool loop = words > share * most || (long long)p.C * p.HW > 0x7fffffffLL;
+    if (loop) share = 16;
+    p.group = share;
+    const int warps = std::max(8, share), per_block = warps / share;
+    const long long blocks = cdivll(tiles, per_block);
     if (blocks > 0x7fffffffLL) return WG2X2_ERR_UNSUPPORTED;
-    const int words = cdiv(p.C, 4);
-    const size_t smem = (size_t)32 * (words | 1) * 4;
-    if (words <= 16) return launch(nchw_kernel<T, MODE, 2>, dim3((unsigned)blocks), 256, smem, st, p);
-    if (words <= 32) return launch(nchw_kernel<T, MODE, 4>, dim3((unsigned)blocks), 256, smem, st, p);
-    if (words <= 64) return launch(nchw_kernel<T, MODE, 8>, dim3((unsigned)blocks), 256, smem, st, p);
-    if (words <= 128) return launch(nchw_kernel<T, MODE, 8>, dim3((unsigned)blocks), 512, smem, st, p);
-    if (words <= 256) return launch(nchw_kernel<T, MODE, 16>, dim3((unsigned)blocks), 512, smem, st, p);
-    return launch(nchw_kernel<T, MODE, 0>, dim3((unsigned)blocks), 512, 0, st, p);
+    const bool by16 = p.C % 16 == 0 && p.ldq % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Q) & 15u) == 0;
+    const int pieces = by16 ? words / 4 : words;
+    p.inv = pieces > 1 ? (unsigned)((0x100000000ull + pieces - 1) / pieces) : 0;       // i / pieces exact for i * pieces < 2^32
+    const size_t smem = (size_t)per_block * 32 * (words | 1) * 4;
+    const int nq = cdiv(words, share);
+    if (loop) return launch(nchw_kernel<T, MODE, 0>, dim3((unsigned)blocks), 32 * warps, 0, st, p);
+    if (nq <= 2) return launch(nchw_kernel<T, MODE, 2>, dim3((unsigned)blocks), 32 * warps, smem, st, p);
+    if (nq <= 4) return launch(nchw_kernel<T, MODE, 4>, dim3((unsigned)blocks), 32 * warps, smem, st, p);
+    if (nq <= 8) return launch(nchw_kernel<T, MODE, 8>, dim3((unsigned)blocks), 32 * warps, smem, st, p);
+    return launch(nchw_kernel<T, MODE, 16>, dim3((unsigned)blocks), 32 * warps, smem, st, p);
 }
 
 static int codes_int8(int mode, int type, RowsParams &p, long long B, int HW, int C, int layout, cudaStream_t st)

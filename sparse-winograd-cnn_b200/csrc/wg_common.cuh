@@ -249,7 +249,7 @@ inline bool grant_smem(const void *kernel, size_t bytes)
 template <typename... KernelArgs, typename... Args>
 int launch_cluster(void (*kernel)(KernelArgs...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t st, Args &&...args)
 {
-    if (smem > 48 * 1024 && !grant_smem(reinterpret_cast<const void *>(kernel), smem)) return WG2X2_ERR_LAUNCH;
+    if (smem > 40 * 1024 && !grant_smem(reinterpret_cast<const void *>(kernel), smem)) return WG2X2_ERR_LAUNCH;
     static const bool pdl_env = [] { const char *e = getenv("WG2X2_PDL"); return !(e && e[0] == '0'); }();
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(st, &capturing) != cudaSuccess) return WG2X2_ERR_LAUNCH;

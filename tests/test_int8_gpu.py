@@ -70,7 +70,9 @@ def _equal(x, y):
 
 
 SIZES = [(1, 1), (3, 2), (21, 7), (40, 8), (25, 16), (301, 17), (64, 33), (21, 63), (1000, 64), (30, 65), (33, 127), (21, 128), (21, 250), (700, 256), (23, 257), (21, 512),
-         (22, 513), (500, 1000), (499, 1001), (21, 1024), (400, 1025), (1, 4096), (321, 4096), (300, 4099), (22, 8192), (2, 12345), (21, 16384), (300, 20001), (21, 40000)]
+         (22, 513), (500, 1000), (499, 1001), (21, 1024), (400, 1025), (1, 4096), (321, 4096), (300, 4099), (22, 8192), (2, 12345), (21, 16384), (300, 20001), (21, 40000),
+         # many rows: blocks that go on to further ones
+         (200001, 4), (100003, 9), (70001, 64), (60000, 33), (20011, 100), (30000, 128), (12345, 250), (9001, 513), (5003, 1001), (3001, 2049), (4000, 4096), (1501, 8192), (700, 16383)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
