@@ -142,26 +142,26 @@ __device__ __forceinline__ Pack load_pack(const T *p, int c0, int C, const T *lo
     }
     return r;
 }
-// The same on its way to shared memory (dst, and `at`, its address there), for the thread that asks for it; nothing for c0 >= C
-template <typename T, int N, bool ODD>
-__device__ __forceinline__ void fetch_pack(uint4 *dst, uint32_t at, const T *p, int c0, int C, const T *lo, const T *hi)
+// The same on its way to shared memory (dst, and `at`, its address there); nothing for c0 >= C.  safe: all of it lies within the tensor.
+template <typename T, int N>
+__device__ __forceinline__ void fetch_pack(uint4 *dst, uint32_t at, const T *p, int c0, int C, bool safe, const T *lo, const T *hi)
 {
     if (c0 >= C) return;
-    if (!ODD || (p + c0 >= lo && p + c0 + N <= hi)) {
+    if (safe || (p + c0 >= lo && p + c0 + N <= hi)) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(p + c0) : "memory");
     } else {
-        const Pack r = load_pack<T, N, ODD>(p, c0, C, lo, hi);
+        const Pack r = load_pack<T, N, true>(p, c0, C, lo, hi);
         *dst = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
     }
 }
-// What a piece has of its neighbours' values becomes zero
+// What lies behind a row's end becomes zero
 template <typename T, int N>
 __device__ __forceinline__ void clear_outside(Pack &r, int c0, int C)
 {
-    if (c0 < 0 || c0 + N > C) {
+    if (c0 + N > C) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (c0 + j < 0 || c0 + j >= C) r.w[j * 4 / N] &= N == 8 ? (j & 1 ? 0x0000ffffu : 0xffff0000u) : 0u;
+            if (c0 + j >= C) r.w[j * 4 / N] &= N == 8 ? (j & 1 ? 0x0000ffffu : 0xffff0000u) : 0u;
     }
 }
 template <typename T, int N, bool ODD>
@@ -203,13 +203,24 @@ __device__ __forceinline__ void load_weights(const RowsParams &p, int c0, float 
     }
 }
 
-__device__ __noinline__ unsigned exact_code(float u, float a) { return (unsigned)__double2int_rn((double)u * 127.0 / (double)a); }
+// The whole number nearest to 127 u / a where u inv, which is within 7.6e-6 of that, is close to half way between two: k + 1/2.  127 u and
+// (k + 1/2) a are compared as sums of two 32-bit numbers each: the high parts lie within a factor of two of each other and the low
+// ones have 8 bits, so every difference is exact.  Both sides are first scaled to where nothing overflows or is denormal.
+__device__ __noinline__ unsigned near_tie(float u, float inv, float a)
+{
+    const float k = floorf(__fmul_rn(u, inv)), half = k + 0.5f, s = a >= 2.f ? 0x1p-64f : 0x1p64f;
+    u *= s;
+    a *= s;
+    const float p = __fmul_rn(127.f, u), q = __fmul_rn(half, a);
+    const float d = __fadd_rn(__fsub_rn(p, q), __fsub_rn(fmaf(127.f, u, -p), fmaf(half, a, -q)));
+    const int i = (int)k;
+    return (unsigned)(d > 0.f || (d == 0.f && (i & 1)) ? i + 1 : i);
+}
 
 // Codes of N values, four a word.  inv = 127 / a rounded, so |u inv - 127 u / a| <= 127 * 2^-24 = 7.6e-6.  m holds the whole number
 // nearest to u inv, which the fused multiply-add rounds once; d, its distance, is exact to 3e-8.  Wherever |d| <= 0.49999 that number is
-// also the one nearest to 127 u / a.  Elsewhere (u = a / 2 is common in 16-bit types) the quotient is taken in 64 bits: 127 u is exact
-// there, and a quotient that is not half way differs from it by more than 2^-33.  a below kTinyRow or not finite: inv = 0, and the
-// caller clears the codes.
+// also the one nearest to 127 u / a; elsewhere near_tie says (u = a / 2 is common in 16-bit types, and there are rows with a tie in every
+// dozen values).  a below kTinyRow or not finite: inv = 0, and the caller clears the codes.
 template <int N>
 __device__ __forceinline__ void code_words(const float (&u)[N], float inv, float a, unsigned (&w)[N / 4])
 {
@@ -227,12 +238,10 @@ __device__ __forceinline__ void code_words(const float (&u)[N], float inv, float
     }
     if (off > kNearTie) {
 #pragma unroll
-        for (int g = 0; g < N / 4; ++g) {
-            unsigned c = 0;
-#pragma unroll 1
-            for (int j = 0; j < 4; ++j)
-                c |= (exact_code(j == 0 ? u[4 * g] : j == 1 ? u[4 * g + 1] : j == 2 ? u[4 * g + 2] : u[4 * g + 3], a) & 0xffu) << (8 * j);
-            w[g] = c;
+        for (int j = 0; j < N; ++j) {
+            const float x = u[j], m = fmaf(x, inv, kRound);
+            if (fabsf(fmaf(x, inv, -__fsub_rn(m, kRound))) > kNearTie)
+                w[j / 4] = __byte_perm(w[j / 4], near_tie(x, inv, a), (j & 3) == 0 ? 0x3214 : (j & 3) == 1 ? 0x3240 : (j & 3) == 2 ? 0x3410 : 0x4210);
         }
     }
 }
@@ -300,16 +309,17 @@ __device__ __forceinline__ void reduce_block(float &a, float &ss, float2 *part)
 // AHEAD: a block has several rows (or blocks of rows) in turn, and the loads of the next AHEAD of them are on their way to shared memory
 // while it works on one.  Every thread fetches the pieces that it uses itself, so nothing waits for other threads.
 // ODD: rows that do not begin on 16 bytes, or whose length is not a multiple; x, shortcut and sum have the same offset to a 16-byte
-// boundary in every row.  Loads are then of the aligned pieces that a row touches, and codes reach their own 4 or 8 bytes by a shift
-// with the next lane's.
+// boundary in every row.  The aligned pieces that a row touches come to shared memory; there the shortcut is added to them, and every
+// thread then reads its N channels at the offset that the row has.
 template <typename T, int MODE, int V, bool BLOCK, bool ODD, int AHEAD>
 __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kernel(const RowsParams p)
 {
-    constexpr int N = 16 / sizeof(T), WORDS = N / 4, PIECES = MODE == kNormRes ? 2 * V : V, STAGES = AHEAD + 1;
+    constexpr int N = 16 / sizeof(T), WORDS = N / 4, STAGES = AHEAD + 1;
     constexpr bool SUM = MODE != kQuantize;
-    extern __shared__ uint4 ring[];                     // [STAGES][PIECES][thread], then the weights of the thread's pieces
+    // [STAGES][x, shortcut][V][thread], ODD: [STAGES][x, shortcut][row][V * threads of a row + 1]; then the weights of the thread's channels
+    extern __shared__ uint4 ring[];
     __shared__ float2 part[BLOCK ? 3 * 32 : 1];
-    constexpr bool W_AT_HAND = SUM && AHEAD && !ODD;    // (ODD: which channels a piece has depends on the row)
+    constexpr bool W_AT_HAND = SUM && AHEAD;
     wait_for_previous_kernel(kNumSMs);
     const int lane = threadIdx.x & 31;
     const int width = BLOCK ? 32 : p.group, at = lane & (width - 1);
@@ -326,18 +336,23 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kern
     T *h = static_cast<T *>(p.H) + (first + mine) * p.ldh;
     signed char *q = p.Q + (first + mine) * p.ldq;
     const long long x_step = stride * p.ldx, r_step = stride * p.ldr, h_step = stride * p.ldh, q_step = stride * p.ldq;
-    const uint32_t slot = 16u * blockDim.x, mine_at = (uint32_t)__cvta_generic_to_shared(ring) + 16u * threadIdx.x;
-    uint4 *const mine_ring = ring + threadIdx.x;
+    // piece v of the thread, of stage s: ring[s * stage + v * slot + mine_in], the shortcut's at + half
+    const int in_row = (BLOCK ? (int)blockDim.x : p.group) * V;
+    const int slot = ODD ? width : blockDim.x, mine_in = ODD ? mine * (in_row + 1) + i0 : threadIdx.x;
+    const int half = ODD ? per_block * (in_row + 1) : V * blockDim.x, stage = MODE == kNormRes ? 2 * half : half;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     long long next = first;
     int put = 0, get = 0, turn = 0;
     auto fetch = [&] {                  // the loads of the block's row `next`, to stage `put`
         if (next < p.rows && (BLOCK || next + mine < p.rows)) {
-            const int mis = offset(xf), k = put * PIECES;
+            const int mis = offset(xf), at0 = put * stage + mine_in;
+            // (whether every piece of the row lies within the tensors)
+            const bool safe = !ODD || (xf - N >= X && xf + p.C + N <= x_end && (MODE != kNormRes || (rf - N >= R && rf + p.C + N <= r_end)));
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const int c0 = (i0 + v * width) * N - mis;
-                fetch_pack<T, N, ODD>(mine_ring + (k + v) * blockDim.x, mine_at + (k + v) * slot, xf, c0, p.C, X, x_end);
-                if (MODE == kNormRes) fetch_pack<T, N, ODD>(mine_ring + (k + V + v) * blockDim.x, mine_at + (k + V + v) * slot, rf, c0, p.C, R, r_end);
+                const int c0 = (i0 + v * width) * N - mis, o = at0 + v * slot;
+                fetch_pack<T, N>(ring + o, ring_at + 16u * o, xf, c0, p.C, safe, X, x_end);
+                if (MODE == kNormRes) fetch_pack<T, N>(ring + o + half, ring_at + 16u * (o + half), rf, c0, p.C, safe, R, r_end);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -346,7 +361,7 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kern
         if (MODE == kNormRes) rf += r_step;
         put = put + 1 < STAGES ? put + 1 : 0;
     };
-    float4 *const weights = reinterpret_cast<float4 *>(ring + STAGES * PIECES * blockDim.x) + threadIdx.x;
+    float4 *const weights = reinterpret_cast<float4 *>(ring + STAGES * stage) + threadIdx.x;
     if (AHEAD) {
         for (int s = 0; s < AHEAD; ++s) fetch();
         if (W_AT_HAND)
@@ -364,28 +379,55 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kern
         const int C = have ? p.C : -N;                  // (nothing of a row that is not there)
         const int mis = offset(x);
         float u[V][N];
-        if (AHEAD) {
+        if (ODD && !BLOCK) __syncwarp();                // the stage that is fetched into has been read by all lanes
+        if (AHEAD || ODD) {
             fetch();
             asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
         }
+        uint4 *const got = ring + get * stage + mine_in;
+        if (ODD) {
+            if (MODE == kNormRes) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const int c0 = (i0 + v * width) * N - mis;
+                    if (c0 >= C) continue;
+                    const Pack sum = Types<T>::sum(pack_at(got + v * slot), pack_at(got + v * slot + half));
+                    store_pack<T, N, true>(h, c0, C, sum);
+                    got[v * slot] = make_uint4(sum.w[0], sum.w[1], sum.w[2], sum.w[3]);
+                }
+            }
+            if (BLOCK) __syncthreads();
+            else __syncwarp();
+        }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int c0 = (i0 + v * width) * N - mis;
-            Pack a = {{0, 0, 0, 0}}, b = a;
-            if (AHEAD) {
+            const int c0 = (i0 + v * width) * N;
+            Pack a = {{0, 0, 0, 0}};
+            if (ODD) {
                 if (c0 < C) {
-                    a = pack_at(mine_ring + (get * PIECES + v) * blockDim.x);
-                    if (MODE == kNormRes) b = pack_at(mine_ring + (get * PIECES + V + v) * blockDim.x);
+                    const unsigned *word = reinterpret_cast<const unsigned *>(got + v * slot) + mis * (int)sizeof(T) / 4;
+                    unsigned t[5];
+#pragma unroll
+                    for (int j = 0; j < 5; ++j) t[j] = j < 4 || N == 8 ? word[j] : 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a.w[j] = N == 8 ? __funnelshift_r(t[j], t[j + 1], 16 * (mis & 1)) : t[j];
                 }
+                clear_outside<T, N>(a, c0, C);
             } else {
-                a = load_pack<T, N, ODD>(x, c0, C, X, x_end);
-                if (MODE == kNormRes) b = load_pack<T, N, ODD>(r, c0, C, R, r_end);
-            }
-            if (ODD) clear_outside<T, N>(a, c0, C);
-            if (MODE == kNormRes) {
-                if (ODD) clear_outside<T, N>(b, c0, C);
-                a = Types<T>::sum(a, b);
-                store_pack<T, N, ODD>(h, c0, C, a);
+                Pack b = a;
+                if (AHEAD) {
+                    if (c0 < C) {
+                        a = pack_at(got + v * slot);
+                        if (MODE == kNormRes) b = pack_at(got + v * slot + half);
+                    }
+                } else {
+                    a = load_pack<T, N, false>(x, c0, C, X, x_end);
+                    if (MODE == kNormRes) b = load_pack<T, N, false>(r, c0, C, R, r_end);
+                }
+                if (MODE == kNormRes) {
+                    a = Types<T>::sum(a, b);
+                    store_pack<T, N, false>(h, c0, C, a);
+                }
             }
             Types<T>::open(a, u[v]);
         }
@@ -402,7 +444,7 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kern
                         w[j] = t.x; w[j + 1] = t.y; w[j + 2] = t.z; w[j + 3] = t.w;
                     }
                 } else {
-                    load_weights<T, N>(p, (i0 + v * width) * N - mis, w);
+                    load_weights<T, N>(p, (i0 + v * width) * N, w);
                 }
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
@@ -427,8 +469,8 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kern
 #pragma unroll 1
                 for (int v = 0; v < V; ++v)
                     for (int j = 0; j < N; ++j) {
-                        const int c = (i0 + v * width) * N - mis + j;
-                        if (c < 0 || c >= C) continue;
+                        const int c = (i0 + v * width) * N + j;
+                        if (c >= C) continue;
                         const float f = to_f(MODE == kNormRes ? h[c] : x[c]) * kDown;
                         s2 = fmaf(f, f, s2);
                     }
@@ -452,54 +494,17 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kern
 #pragma unroll
             for (int g = 0; g < WORDS; ++g) w[v][g] &= k.live;
         }
-        if (!ODD) {
+        const bool whole = !ODD || (reinterpret_cast<uintptr_t>(q) & (N - 1)) == 0;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int c0 = (i0 + v * width) * N;
-                if (c0 < C) {
-                    if (WORDS == 2) *reinterpret_cast<uint2 *>(q + c0) = make_uint2(w[v][0], w[v][WORDS - 1]);
-                    else *reinterpret_cast<unsigned *>(q + c0) = w[v][0];
-                }
-            }
-        } else {
-            // Piece i has the codes of channels i N - mis .. i N - mis + N - 1; with the first mis of the next piece, those of i N .. i N + N - 1.
-            // The last piece of a warp's (or group's) has no next one at hand and stores what it has; the first stores what lies in front.
-            const bool whole = (reinterpret_cast<uintptr_t>(q) & (N - 1)) == 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                unsigned s[2 * WORDS + 1];
-#pragma unroll
-                for (int g = 0; g < WORDS; ++g) {
-                    s[g] = w[v][g];
-                    s[WORDS + g] = __shfl_down_sync(0xffffffffu, w[v][g], 1);
-                    if (v + 1 < V) {
-                        const unsigned wrapped = __shfl_sync(0xffffffffu, w[v + 1 < V ? v + 1 : v][g], lane & ~(width - 1));
-                        if (at == width - 1) s[WORDS + g] = wrapped;
-                    }
-                }
-                s[2 * WORDS] = 0;
-                const bool next = v + 1 < V || at < width - 1;
-                const int c0 = (i0 + v * width) * N, count = min(next ? N : N - mis, C - c0);
-                unsigned o[WORDS];
-#pragma unroll
-                for (int g = 0; g < WORDS; ++g) {
-                    const bool far = WORDS == 2 && (mis & 4);
-                    o[g] = __funnelshift_r(far ? s[g + 1] : s[g], far ? s[g + 2] : s[g + 1], 8 * (mis & 3));
-                }
-                if (count == N && whole) {
-                    if (WORDS == 2) *reinterpret_cast<uint2 *>(q + c0) = make_uint2(o[0], o[WORDS - 1]);
-                    else *reinterpret_cast<unsigned *>(q + c0) = o[0];
-                } else if (count > 0) {
-#pragma unroll
-                    for (int j = 0; j < N; ++j)
-                        if (j < count) q[c0 + j] = (signed char)(o[j >> 2] >> (8 * (j & 3)));
-                }
-            }
-            if (BLOCK && i0 > 0 && lane == 0) {
-                const int c0 = i0 * N - mis;
+        for (int v = 0; v < V; ++v) {
+            const int c0 = (i0 + v * width) * N;
+            if (ODD ? c0 + N <= C && whole : c0 < C) {
+                if (WORDS == 2) *reinterpret_cast<uint2 *>(q + c0) = make_uint2(w[v][0], w[v][WORDS - 1]);
+                else *reinterpret_cast<unsigned *>(q + c0) = w[v][0];
+            } else if (ODD && c0 < C) {
 #pragma unroll
                 for (int j = 0; j < N; ++j)
-                    if (j < mis && c0 + j < C) q[c0 + j] = (signed char)(w[0][j >> 2] >> (8 * (j & 3)));
+                    if (c0 + j < C) q[c0 + j] = (signed char)(w[v][j >> 2] >> (8 * (j & 3)));
             }
         }
         x += x_step;
@@ -736,7 +741,8 @@ template <typename T, int MODE, int V, bool BLOCK, bool ODD, int AHEAD>
 static int launch_rows(int threads, const RowsParams &p, cudaStream_t st)
 {
     auto *kernel = rows_kernel<T, MODE, V, BLOCK, ODD, AHEAD>;
-    const size_t smem = AHEAD ? (size_t)((AHEAD + 1) * (MODE == kNormRes ? 2 * V : V) * 16 + (MODE != kQuantize && !ODD ? V * (16 / (int)sizeof(T)) * 4 : 0)) * threads : 0;
+    const int tensors = MODE == kNormRes ? 2 : 1, pieces = ODD ? V * threads + (BLOCK ? 1 : threads / p.group) : V * threads;
+    const size_t smem = (AHEAD || ODD ? (size_t)(AHEAD + 1) * tensors * pieces * 16 : 0) + (AHEAD && MODE != kQuantize ? (size_t)V * (16 / sizeof(T)) * 4 * threads : 0);
     long long blocks = cdivll(p.rows, BLOCK ? 1 : threads / p.group);
     if (AHEAD) {
         static const int regs = [&] {
