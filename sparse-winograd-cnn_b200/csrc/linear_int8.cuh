@@ -16,7 +16,8 @@ constexpr int kLiThreads = 320;               // producer, MMA issuer, eight epi
 constexpr int kLiChunk = 128;                 // bytes of the contraction a stage
 constexpr int kLiMaxStages = 12;
 constexpr int kLiSmem = 232448;               // all that a CTA can have
-constexpr int kLiCtrl = 512 + 8 * 64 * 4;     // barriers; 32 column scales and 32 biases for each epilogue warp
+constexpr int kLiCorner = 128;                // columns of a tile that an epilogue warp finishes, at most
+constexpr int kLiCtrl = 512 + 8 * 2 * kLiCorner * 4;     // barriers; the scales and biases of those columns, for each epilogue warp
 constexpr int kLiMaxC = 131071;
 
 struct LiParams {
@@ -87,11 +88,13 @@ template <> __device__ __forceinline__ float li_out<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half li_out<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 li_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// (the weights' scale first: of the two it is the one of ordinary size; without a bias the sum is with -0, which changes nothing)
-__device__ __forceinline__ float li_value(int acc, float w_scale, float q_scale, float bias, bool relu)
+// (The weights' scale first: of the two it is the one of ordinary size.  Without a bias the sum is with -0, which changes nothing; low = 0
+// for a ReLU, which keeps NaN, and -infinity for none.)
+__device__ __forceinline__ float li_value(int acc, float w_scale, float q_scale, float bias, float low)
 {
-    const float v = fmaf(__fmul_rn((float)acc, w_scale), q_scale, bias);
-    return relu ? relu_nan(v) : v;
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fmaf(__fmul_rn((float)acc, w_scale), q_scale, bias)), "f"(low));
+    return r;
 }
 
 // 16 lane tiles x all column tiles at a time, so that the CTAs that run together share operands in L2
@@ -102,12 +105,12 @@ __device__ __forceinline__ void li_decode(const LiParams &p, int u, int &lt, int
     lt = 16 * group + r - ct * size;
 }
 
-// What a thread knows about its lane of a tile
+// An epilogue thread's share of a tile: its lane (row of A) with all of the warp's columns
 template <bool NCHW, typename T>
 struct LiLane {
     T *dst;                     // Y at column 0
     long long step;             // elements from column to column
-    float scale, bias;
+    float scale, bias, low;
     bool live;
     __device__ __forceinline__ LiLane(const LiParams &p, int lane_row)
     {
@@ -115,6 +118,7 @@ struct LiLane {
         const int r = live ? lane_row : 0;
         scale = p.lane_scale[r];
         bias = !NCHW && p.bias ? p.bias[r] : -0.f;
+        low = p.relu ? 0.f : __uint_as_float(0xff800000u);
         if (NCHW) {
             const int b = r / p.HW;
             dst = static_cast<T *>(p.Y) + (long long)b * p.K * p.HW + (r - b * p.HW);
@@ -125,16 +129,63 @@ struct LiLane {
         }
     }
 };
-
-// Scales (and biases) of 32 columns, in the warp's corner of shared memory
+// Scales (and biases) of a warp's columns, 32 a time one a lane: asked for while the tile before is stored, then put where all lanes read them
 template <bool NCHW>
-__device__ __forceinline__ void li_stage_columns(const LiParams &p, float *corner, int col0, int lane)
+struct LiColumns {
+    float scale[kLiCorner / 32], bias[kLiCorner / 32];
+    __device__ __forceinline__ void load(const LiParams &p, int col0, int ncols, int lane)
+    {
+#pragma unroll
+        for (int k = 0; k < kLiCorner / 32; ++k) {
+            const int c = col0 + 32 * k + lane;
+            const bool ok = 32 * k < ncols && c < p.cols;
+            scale[k] = ok ? p.col_scale[c] : 0.f;
+            bias[k] = NCHW && ok && p.bias ? p.bias[c] : -0.f;
+        }
+    }
+    __device__ __forceinline__ void put(float *corner, int lane) const
+    {
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < kLiCorner / 32; ++k) {
+            corner[32 * k + lane] = scale[k];
+            if (NCHW) corner[kLiCorner + 32 * k + lane] = bias[k];
+        }
+        __syncwarp();
+    }
+};
+template <bool NCHW, typename T, bool WHOLE>
+__device__ __forceinline__ void li_store32(const LiLane<NCHW, T> &me, const int (&r)[32], const float *corner, T *dst, int n)
 {
-    const int c = col0 + lane;
-    __syncwarp();
-    corner[lane] = c < p.cols ? p.col_scale[c] : 0.f;
-    if (NCHW) corner[32 + lane] = c < p.cols && p.bias ? p.bias[c] : -0.f;
-    __syncwarp();
+#pragma unroll
+    for (int x4 = 0; x4 < 8; ++x4) {
+        const float4 cs4 = *reinterpret_cast<const float4 *>(corner + 4 * x4);
+        const float4 cb4 = NCHW ? *reinterpret_cast<const float4 *>(corner + kLiCorner + 4 * x4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float cs[4] = {cs4.x, cs4.y, cs4.z, cs4.w}, cb[4] = {cb4.x, cb4.y, cb4.z, cb4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int x = 4 * x4 + j;
+            const float v = NCHW ? li_value(r[x], cs[j], me.scale, cb[j], me.low) : li_value(r[x], me.scale, cs[j], me.bias, me.low);
+            if (WHOLE || (me.live && x < n)) *dst = li_out<T>(v);
+            dst += me.step;
+        }
+    }
+}
+// ncols columns (at most kLiCorner) from tensor memory at taddr, the first being column col0 of the result
+template <bool NCHW, typename T>
+__device__ __forceinline__ void li_store(const LiParams &p, const LiLane<NCHW, T> &me, uint32_t taddr, const float *corner, int col0, int ncols)
+{
+    const int have = min(ncols, p.cols - col0);
+    const bool live = __all_sync(0xffffffffu, me.live);
+    T *dst = me.dst + col0 * me.step;
+    for (int c = 0; c < have; c += 32) {
+        int r[32];
+        tmem_ld32(taddr + (uint32_t)c, r);
+        tmem_wait32(r);
+        if (live && have - c >= 32) li_store32<NCHW, T, true>(me, r, corner + c, dst, 32);
+        else li_store32<NCHW, T, false>(me, r, corner + c, dst, have - c);
+        dst += 32 * me.step;
+    }
 }
 
 // SPLIT: one tile per cluster of `splits` CTAs, else the CTA's tiles in turn
@@ -175,7 +226,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
     wait_for_previous_kernel(kNumSMs);
 
     const int rank = SPLIT ? (int)cluster_ctarank() : 0;
-    const int first = SPLIT ? blockIdx.x / prm.splits : blockIdx.x, step = SPLIT ? 1 << 30 : gridDim.x;
+    const int first = SPLIT ? blockIdx.x / prm.splits : blockIdx.x, step = SPLIT ? 1 << 30 : (int)gridDim.x;
     const int units = prm.lane_tiles * prm.col_tiles;
     // (at least one chunk for every CTA: splits <= chunks)
     const int kbeg = SPLIT ? rank * prm.chunks / prm.splits : 0, kend = SPLIT ? (rank + 1) * prm.chunks / prm.splits : prm.chunks;
@@ -234,46 +285,32 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
         if (!ok) let_them_land();
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;
-        float *corner = reinterpret_cast<float *>(ctrl_gen + 512) + (warp - 2) * 64;
+        float *corner = reinterpret_cast<float *>(ctrl_gen + 512) + (warp - 2) * 2 * kLiCorner;
         const uint32_t quarter = (uint32_t)(q * 32) << 16;
         int buf = 0;
         uint32_t use = 0;
         if (!SPLIT) {
-            const int ncols = prm.N >= 64 ? prm.N / 2 : prm.N;          // columns of a warp (N = 32: those of half 0)
+            const int ncols = prm.N >= 64 ? prm.N / 2 : half ? 0 : prm.N, c_tile = prm.N >= 64 ? half * ncols : 0;      // the warp's columns of a tile
+            int lt, ct;
+            li_decode(prm, min(first, units - 1), lt, ct);
+            LiLane<NCHW, T> me(prm, lt * kBlockM + q * 32 + lane);
+            LiColumns<NCHW> columns;
+            columns.load(prm, ct * prm.N + c_tile, ncols, lane);
             for (int u = first; u < units; u += step) {
-                int lt, ct;
-                li_decode(prm, u, lt, ct);
-                const LiLane<NCHW, T> me(prm, lt * kBlockM + q * 32 + lane);
-                const int c_first = ct * prm.N + (prm.N >= 64 ? half * ncols : 0);
+                const int col0 = ct * prm.N + c_tile;
+                columns.put(corner, lane);
+                li_decode(prm, min(u + step, units - 1), lt, ct);
+                const LiLane<NCHW, T> next(prm, lt * kBlockM + q * 32 + lane);
+                columns.load(prm, ct * prm.N + c_tile, ncols, lane);
                 if (!mbar_wait_warp(accf_bar(buf), use & 1u, abort_flag, 0x1F00u | buf, prm.spin_limit)) { ok = false; break; }
                 tc_fence_after();
-                for (int cc = 0; cc < ncols && (prm.N >= 64 || half == 0); cc += 32) {
-                    const int col0 = c_first + cc;
-                    if (col0 >= prm.cols) break;
-                    int r[32];
-                    tmem_ld32(tmem_base + quarter + (uint32_t)(buf * 256 + (prm.N >= 64 ? half * ncols : 0) + cc), r);
-                    li_stage_columns<NCHW>(prm, corner, col0, lane);
-                    tmem_wait32(r);
-                    T *dst = me.dst + col0 * me.step;
-                    const int n = min(min(32, ncols - cc), prm.cols - col0);
-#pragma unroll
-                    for (int x4 = 0; x4 < 8; ++x4) {
-                        const float4 cs4 = *reinterpret_cast<const float4 *>(corner + 4 * x4);
-                        const float4 cb4 = NCHW ? *reinterpret_cast<const float4 *>(corner + 32 + 4 * x4) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        const float cs[4] = {cs4.x, cs4.y, cs4.z, cs4.w}, cb[4] = {cb4.x, cb4.y, cb4.z, cb4.w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int x = 4 * x4 + j;
-                            const float v = NCHW ? li_value(r[x], cs[j], me.scale, cb[j], prm.relu) : li_value(r[x], me.scale, cs[j], me.bias, prm.relu);
-                            if (me.live && x < n) dst[x * me.step] = li_out<T>(v);
-                        }
-                    }
-                }
+                li_store<NCHW, T>(prm, me, tmem_base + quarter + (uint32_t)(buf * 256 + c_tile), corner, col0, ncols);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(acce_bar(buf));
                 buf ^= 1;
                 if (buf == 0) ++use;
+                me = next;
             }
         } else {
             // this CTA's share of the sums to the CTAs that finish them: [share][column][lane]
@@ -312,7 +349,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
                 int acc = 0;
                 for (int s = 0; s < prm.splits; ++s) acc += sums[(s * mine + c) * kBlockM];
                 const float cs = prm.col_scale[col], b = NCHW ? (prm.bias ? prm.bias[col] : -0.f) : me.bias;
-                const float v = NCHW ? li_value(acc, cs, me.scale, b, prm.relu) : li_value(acc, me.scale, cs, b, prm.relu);
+                const float v = NCHW ? li_value(acc, cs, me.scale, b, me.low) : li_value(acc, me.scale, cs, b, me.low);
                 if (me.live) me.dst[col * me.step] = li_out<T>(v);
             }
         }
