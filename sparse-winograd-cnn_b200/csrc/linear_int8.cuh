@@ -12,12 +12,14 @@
 // the shares (whole numbers, so the order does not matter) meet through distributed shared memory, every CTA finishing N / S columns.
 #pragma once
 
-constexpr int kLiThreads = 320;               // producer, MMA issuer, eight epilogue warps
+constexpr int kLiEpiWarps = 16;               // four for each quarter of the lanes: a product with few channels is all epilogue
+constexpr int kLiThreads = 32 * (2 + kLiEpiWarps);       // producer, MMA issuer, epilogue
 constexpr int kLiChunk = 128;                 // bytes of the contraction a stage
 constexpr int kLiMaxStages = 12;
 constexpr int kLiSmem = 232448;               // all that a CTA can have
-constexpr int kLiCorner = 128;                // columns of a tile that an epilogue warp finishes, at most
-constexpr int kLiCtrl = 512 + 8 * 2 * kLiCorner * 4;     // barriers; the scales and biases of those columns, for each epilogue warp
+constexpr int kLiAhead = 4;
+constexpr int kLiCorner = 64;                 // columns of a tile that an epilogue warp finishes, at most
+constexpr int kLiCtrl = 512 + kLiEpiWarps * 2 * kLiCorner * 4;     // barriers; the scales and biases of those columns, for each epilogue warp
 constexpr int kLiMaxC = 131071;
 
 struct LiParams {
@@ -27,7 +29,7 @@ struct LiParams {
     int lanes, cols;                                // rows of A and of B
     int K, HW;                                      // NCHW: channels and pixels of Y's images
     int N, stages, chunks;                          // columns of a tile; stages of operands; chunks of the contraction
-    int lane_tiles, col_tiles, splits, relu;
+    int lane_tiles, col_tiles, splits, pair, relu;
     uint32_t spin_limit;
     int drop_load;
 };
@@ -100,27 +102,37 @@ __device__ __forceinline__ float li_value(int acc, float w_scale, float q_scale,
 // 16 lane tiles x all column tiles at a time, so that the CTAs that run together share operands in L2
 __device__ __forceinline__ void li_decode(const LiParams &p, int u, int &lt, int &ct)
 {
+    if (p.col_tiles == 1) {
+        lt = u;
+        ct = 0;
+        return;
+    }
     const int group = u / (16 * p.col_tiles), r = u - group * 16 * p.col_tiles, size = min(16, p.lane_tiles - 16 * group);
     ct = r / size;
     lt = 16 * group + r - ct * size;
 }
 
 // An epilogue thread's share of a tile: its lane (row of A) with all of the warp's columns
+struct LiScale { float scale, bias; };          // of a lane; the bias where lanes are output channels
+template <bool NCHW>
+__device__ __forceinline__ LiScale li_lane_scale(const LiParams &p, int lane_row)
+{
+    const int r = min(lane_row, p.lanes - 1);
+    return {p.lane_scale[r], !NCHW && p.bias ? p.bias[r] : -0.f};
+}
 template <bool NCHW, typename T>
 struct LiLane {
     T *dst;                     // Y at column 0
     long long step;             // elements from column to column
     float scale, bias, low;
     bool live;
-    __device__ __forceinline__ LiLane(const LiParams &p, int lane_row)
+    __device__ __forceinline__ LiLane(const LiParams &p, int lane_row, const LiScale &s) : scale(s.scale), bias(s.bias)
     {
         live = lane_row < p.lanes;
-        const int r = live ? lane_row : 0;
-        scale = p.lane_scale[r];
-        bias = !NCHW && p.bias ? p.bias[r] : -0.f;
+        const unsigned r = live ? lane_row : 0;
         low = p.relu ? 0.f : __uint_as_float(0xff800000u);
         if (NCHW) {
-            const int b = r / p.HW;
+            const unsigned b = r / (unsigned)p.HW;
             dst = static_cast<T *>(p.Y) + (long long)b * p.K * p.HW + (r - b * p.HW);
             step = p.HW;
         } else {
@@ -188,6 +200,49 @@ __device__ __forceinline__ void li_store(const LiParams &p, const LiLane<NCHW, T
     }
 }
 
+// What an epilogue warp does with the tiles first, first + step, ... of `lanes_tile` lanes; the CTA's begin at lane0 of them.  accf, acce:
+// barriers of the first accumulator, those of the second 8 bytes further; `release` hands an accumulator back.  False: gave up waiting.
+template <bool NCHW, typename T, typename Release>
+__device__ __forceinline__ bool li_epilogue(const LiParams &prm, int first, int step, int lanes_tile, int lane0, int part, int q, int lane, float *corner,
+                                            uint32_t tmem, uint32_t accf, uint32_t acce, volatile int *abort_flag, Release release)
+{
+    const int units = prm.lane_tiles * prm.col_tiles, width = max(32, prm.N / 4);
+    const int c_tile = part * width, ncols = min(width, prm.N - c_tile);         // the warp's columns of a tile (none: ncols <= 0)
+    // A tile with a short contraction takes less time than a load from memory: the lanes' scales are asked for kLiAhead tiles ahead
+    LiScale ahead[kLiAhead];
+    int lt, ct, col_now = -1, buf = 0;
+    uint32_t use = 0;
+#pragma unroll
+    for (int k = 0; k < kLiAhead; ++k) {
+        li_decode(prm, (int)min((long long)units - 1, first + (long long)k * step), lt, ct);
+        ahead[k] = li_lane_scale<NCHW>(prm, lt * lanes_tile + lane0 + q * 32 + lane);
+    }
+    LiColumns<NCHW> columns;
+    for (int u = first; u < units; u += step) {
+        li_decode(prm, u, lt, ct);
+        const LiLane<NCHW, T> me(prm, lt * lanes_tile + lane0 + q * 32 + lane, ahead[0]);
+        const int col0 = ct * prm.N + c_tile;
+#pragma unroll
+        for (int k = 0; k + 1 < kLiAhead; ++k) ahead[k] = ahead[k + 1];
+        if (col0 != col_now) {
+            columns.load(prm, col0, ncols, lane);
+            columns.put(corner, lane);
+            col_now = col0;
+        }
+        li_decode(prm, (int)min((long long)units - 1, u + (long long)kLiAhead * step), lt, ct);
+        ahead[kLiAhead - 1] = li_lane_scale<NCHW>(prm, lt * lanes_tile + lane0 + q * 32 + lane);
+        if (!mbar_wait_warp(accf + 8u * buf, use & 1u, abort_flag, 0x1F00u | buf, prm.spin_limit)) return false;
+        tc_fence_after();
+        li_store<NCHW, T>(prm, me, tmem + (uint32_t)(buf * 256 + c_tile), corner, col0, ncols);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) release(acce + 8u * buf);
+        buf ^= 1;
+        if (buf == 0) ++use;
+    }
+    return true;
+}
+
 // SPLIT: one tile per cluster of `splits` CTAs, else the CTA's tiles in turn
 template <bool NCHW, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kLiThreads, 1)
@@ -210,7 +265,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < prm.stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), kEpiWarps); }
+        for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), kLiEpiWarps); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -284,34 +339,12 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
         }
         if (!ok) let_them_land();
     } else {
-        const int q = warp & 3, half = (warp - 2) >> 2;
+        const int q = warp & 3, part = (warp - 2) >> 2;
         float *corner = reinterpret_cast<float *>(ctrl_gen + 512) + (warp - 2) * 2 * kLiCorner;
         const uint32_t quarter = (uint32_t)(q * 32) << 16;
-        int buf = 0;
-        uint32_t use = 0;
         if (!SPLIT) {
-            const int ncols = prm.N >= 64 ? prm.N / 2 : half ? 0 : prm.N, c_tile = prm.N >= 64 ? half * ncols : 0;      // the warp's columns of a tile
-            int lt, ct;
-            li_decode(prm, min(first, units - 1), lt, ct);
-            LiLane<NCHW, T> me(prm, lt * kBlockM + q * 32 + lane);
-            LiColumns<NCHW> columns;
-            columns.load(prm, ct * prm.N + c_tile, ncols, lane);
-            for (int u = first; u < units; u += step) {
-                const int col0 = ct * prm.N + c_tile;
-                columns.put(corner, lane);
-                li_decode(prm, min(u + step, units - 1), lt, ct);
-                const LiLane<NCHW, T> next(prm, lt * kBlockM + q * 32 + lane);
-                columns.load(prm, ct * prm.N + c_tile, ncols, lane);
-                if (!mbar_wait_warp(accf_bar(buf), use & 1u, abort_flag, 0x1F00u | buf, prm.spin_limit)) { ok = false; break; }
-                tc_fence_after();
-                li_store<NCHW, T>(prm, me, tmem_base + quarter + (uint32_t)(buf * 256 + c_tile), corner, col0, ncols);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(acce_bar(buf));
-                buf ^= 1;
-                if (buf == 0) ++use;
-                me = next;
-            }
+            ok = li_epilogue<NCHW, T>(prm, first, step, kBlockM, 0, part, q, lane, corner, tmem_base + quarter, accf_bar(0), acce_bar(0), abort_flag,
+                                      [](uint32_t bar) { mbar_arrive(bar); });
         } else {
             // this CTA's share of the sums to the CTAs that finish them: [share][column][lane]
             ok = mbar_wait_warp(accf_bar(0), 0, abort_flag, 0x1F00u, prm.spin_limit);
@@ -319,7 +352,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
             if (ok) {
                 const int mine = prm.N / prm.splits;
                 const uint32_t sums = ctrl + kLiCtrl;
-                for (int c8 = half * 8; c8 < prm.N; c8 += 16) {
+                for (int c8 = part * 8; c8 < prm.N; c8 += 32) {
                     int r[8];
                     tmem_ld8i(tmem_base + quarter + (uint32_t)c8, r);
                     tmem_wait8(r);
@@ -340,10 +373,11 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
         if (warp >= 2) {
             int lt, ct;
             li_decode(prm, first, lt, ct);
-            const int q = warp & 3, half = (warp - 2) >> 2, mine = prm.N / prm.splits;
-            const LiLane<NCHW, T> me(prm, lt * kBlockM + q * 32 + lane);
+            const int q = warp & 3, part = (warp - 2) >> 2, mine = prm.N / prm.splits;
+            const int lane_row = lt * kBlockM + q * 32 + lane;
+            const LiLane<NCHW, T> me(prm, lane_row, li_lane_scale<NCHW>(prm, lane_row));
             const int *sums = reinterpret_cast<const int *>(ctrl_gen + kLiCtrl) + q * 32 + lane;
-            for (int c = half; c < mine; c += 2) {
+            for (int c = part; c < mine; c += 4) {
                 const int col = ct * prm.N + rank * mine + c;
                 if (col >= prm.cols) break;
                 int acc = 0;
@@ -358,6 +392,130 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+// The same on pairs of SMs (tcgen05 cta_group::2) for tiles of 256 lanes x N columns: each CTA of a cluster of two has 128 of the lanes and
+// brings half of B, which the tensor cores exchange, so that 256 columns take 32 KB of operands a chunk and SM instead of 48: at one CTA a
+// tile it is the operands' way from L2 that the products wait for.  Barriers as in conv_tc_gemm2.cuh: `full` in the leader counts both
+// CTAs' bytes, `empty` and `accf` are committed to both, `acce` in the leader counts the epilogue warps of both.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t cluster_bar, int c0, int c1)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(cluster_bar), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+template <bool NCHW, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLiThreads, 1)
+linear_int8_pair_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const LiParams prm)
+{
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    const int stage_bytes = (kBlockM + prm.N / 2) * kLiChunk;             // of one CTA
+    const uint32_t ctrl = base + prm.stages * stage_bytes;
+    uint8_t *ctrl_gen = smem_raw + (ctrl - raw);
+    auto full_bar = [&](int s) { return ctrl + 8u * s; };
+    auto empty_bar = [&](int s) { return ctrl + 8u * (kLiMaxStages + s); };
+    auto accf_bar = [&](int b) { return ctrl + 8u * (2 * kLiMaxStages + b); };
+    auto acce_bar = [&](int b) { return ctrl + 8u * (2 * kLiMaxStages + 2 + b); };
+    volatile uint32_t *tmem_ptr_slot = reinterpret_cast<volatile uint32_t *>(ctrl_gen + 8 * (2 * kLiMaxStages + 4));
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(ctrl_gen + 8 * (2 * kLiMaxStages + 5));
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < prm.stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), 2 * kLiEpiWarps); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {       // the same warp of both CTAs, the same slot address
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void *)tmem_ptr_slot)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();    // the partner's barriers exist before anything is signalled into them
+    tc_fence_after();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_slot, 0);
+    wait_for_previous_kernel(kNumSMs);
+
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1, units = prm.lane_tiles * prm.col_tiles;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, loads = 0;
+            uint32_t ph = 0;
+            for (int u = first; u < units && ok; u += step) {
+                int lt, ct;
+                li_decode(prm, u, lt, ct);
+                const int row = lt * 256 + (int)rank * kBlockM, col = ct * prm.N + (int)rank * (prm.N / 2);
+                for (int kc = 0; kc < prm.chunks; ++kc) {
+                    if (loads++ == prm.drop_load && blockIdx.x == 0) { ok = false; break; }
+                    if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, 0x1C00u | s, prm.spin_limit)) { ok = false; break; }
+                    if (rank == 0) mbar_expect_tx(full_bar(s), 2u * stage_bytes);      // both CTAs' tiles land on the leader's barrier
+                    const uint32_t dst = base + s * stage_bytes, bar = mapa_rank0(full_bar(s));
+                    tma_load_2d_pair(dst, &mapA, bar, kc * kLiChunk, row);
+                    tma_load_2d_pair(dst + kBlockM * kLiChunk, &mapB, bar, kc * kLiChunk, col);
+                    if (++s == prm.stages) { s = 0; ph ^= 1u; }
+                }
+            }
+            if (!ok) let_them_land();
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const bool leader = elect_one();
+            const uint32_t idesc = make_idesc_i8(256, prm.N);
+            int s = 0, buf = 0;
+            uint32_t ph = 0, use = 0;
+            for (int u = first; u < units && ok; u += step) {
+                if (!mbar_wait_warp(acce_bar(buf), (use & 1u) ^ 1u, abort_flag, 0x1D00u | buf, prm.spin_limit)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (uint32_t)(buf * 256);
+                for (int kc = 0; kc < prm.chunks; ++kc) {
+                    if (!mbar_wait_warp(full_bar(s), ph, abort_flag, 0x1E00u | s, prm.spin_limit)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t at = base + s * stage_bytes;
+                    const uint64_t ad = make_desc_k_sw128(at), bd = make_desc_k_sw128(at + kBlockM * kLiChunk);
+                    if (leader) {
+#pragma unroll
+                        for (int kk = 0; kk < kLiChunk / 32; ++kk) umma_i8_pair(d_tmem, ad + 2u * kk, bd + 2u * kk, idesc, kc > 0 || kk > 0 ? 1u : 0u);
+                        umma_commit_pair(empty_bar(s));
+                    }
+                    __syncwarp();
+                    if (++s == prm.stages) { s = 0; ph ^= 1u; }
+                }
+                if (ok && leader) umma_commit_pair(accf_bar(buf));
+                __syncwarp();
+                buf ^= 1;
+                if (buf == 0) ++use;
+            }
+            if (!ok) let_them_land();
+        }
+    } else {
+        const int q = warp & 3, part = (warp - 2) >> 2;
+        float *corner = reinterpret_cast<float *>(ctrl_gen + 512) + (warp - 2) * 2 * kLiCorner;
+        li_epilogue<NCHW, T>(prm, first, step, 256, (int)rank * kBlockM, part, q, lane, corner, tmem_base + ((uint32_t)(q * 32) << 16), accf_bar(0), acce_bar(0),
+                             abort_flag, [](uint32_t bar) { mbar_arrive_cluster(mapa_rank0(bar)); });
+    }
+    // Neither CTA may leave, or free its tensor memory, while the other can still read its shared memory through an MMA or signal one of its
+    // barriers
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
     }
 }
 
@@ -380,21 +538,48 @@ static bool make_map_codes(CUtensorMap *map, const void *ptr, int C, long long r
     return r == CUDA_SUCCESS;
 }
 
-// Columns of a tile and CTAs that share one, by an estimate in clocks: a chunk of operands comes from L2 at about 64 bytes a clock and
-// SM, a column of 128 lanes is finished in about 10 clocks (beside the next tile's products, where there is one), and a shared tile
-// costs a cluster's barrier and exchange.
-static void li_choose(LiParams &p)
+// Pairs of SMs that run at once
+static int li_pairs()
+{
+    static std::atomic<int> known[64];           // 0: not asked yet, else the number + 1
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int n = known[dev].load();
+    if (n) return n - 1;
+    auto *kernel = linear_int8_pair_kernel<false, float>;
+    if (grant_smem(reinterpret_cast<const void *>(kernel), kLiSmem)) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(kNumSMs);
+        cfg.blockDim = dim3(kLiThreads);
+        cfg.dynamicSmemBytes = kLiSmem;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { n = 0; (void)cudaGetLastError(); }
+    }
+    known[dev].store(n + 1);
+    return n;
+}
+
+// Columns of a tile, CTAs that share one, and whether pairs of SMs do, by an estimate in clocks: a chunk of operands comes from L2 at about
+// 64 bytes a clock and SM, the tensor cores take 2 clocks for a chunk of a column; a column of 128 lanes is finished in about 10 clocks and
+// a tile in 600 more (beside the next tile's products, where there is one); a shared tile costs a cluster's barrier and exchange.
+static void li_choose(LiParams &p, int pairs)
 {
     double best = 1e300;
+    const int lanes = p.lanes;
     for (int N = 16; N <= 256; N *= 2) {
-        const long long tiles = (long long)p.lane_tiles * cdiv(p.cols, N);
+        const long long cols = cdiv(p.cols, N), tiles = cols * cdiv(lanes, kBlockM);
         for (int S = 1; S <= 8; S *= 2) {
             if (S > 1 && (N > 128 || S > p.chunks || tiles * S > kNumSMs)) break;
-            const double chunk = 2.0 * (kBlockM + N), main = (double)cdiv(p.chunks, S) * chunk, store = 10.0 * N / S;
+            const double main = (double)cdiv(p.chunks, S) * 2 * (kBlockM + N), store = (600 + 10.0 * N) / S;
             const double t = (double)cdivll(tiles * S, kNumSMs) * std::max(main, store) + std::min(main, store) + (S > 1 ? 1000 + 4 * N : 0);
-            if (t < best * 0.999) { best = t; p.N = N; p.splits = S; }
+            if (t < best * 0.999) { best = t; p.N = N; p.splits = S; p.pair = 0; }
+        }
+        if (N >= 128 && pairs > 0) {
+            const double main = (double)p.chunks * std::max(2 * N, 256 + N), store = 600 + 10.0 * N;
+            const double t = (double)cdivll(cols * cdiv(lanes, 256), pairs) * std::max(main, store) + std::min(main, store) + 500;
+            if (t < best * 0.999) { best = t; p.N = N; p.splits = 1; p.pair = 1; }
         }
     }
+    p.lane_tiles = cdiv(lanes, p.pair ? 256 : kBlockM);
     p.col_tiles = cdiv(p.cols, p.N);
 }
 
@@ -406,8 +591,10 @@ static int li_launch(const CUtensorMap &mapA, const CUtensorMap &mapB, const LiP
     return launch_cluster(linear_int8_kernel<NCHW, T, true>, dim3((unsigned)(tiles * p.splits)), p.splits, kLiThreads, smem, st, mapA, mapB, p);
 }
 template <bool NCHW, typename T>
-static int li_launch(const CUtensorMap &mapA, const CUtensorMap &mapB, const LiParams &p, size_t smem, cudaStream_t st)
+static int li_launch(const CUtensorMap &mapA, const CUtensorMap &mapB, const LiParams &p, int pairs, size_t smem, cudaStream_t st)
 {
+    if (p.pair)
+        return launch(linear_int8_pair_kernel<NCHW, T>, dim3(2 * (unsigned)std::min<long long>((long long)p.lane_tiles * p.col_tiles, pairs)), kLiThreads, smem, st, mapA, mapB, p);
     return p.splits > 1 ? li_launch<NCHW, T, true>(mapA, mapB, p, smem, st) : li_launch<NCHW, T, false>(mapA, mapB, p, smem, st);
 }
 
@@ -435,19 +622,19 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     p.lanes = nchw ? (int)rows : K;
     p.cols = nchw ? K : (int)rows;
     p.chunks = cdiv(C, kLiChunk);
-    p.lane_tiles = cdiv(p.lanes, kBlockM);
-    li_choose(p);
+    const int pairs = li_pairs();
+    li_choose(p, pairs);
     if ((long long)p.lane_tiles * p.col_tiles > 0x3fffffffLL) return WG2X2_ERR_UNSUPPORTED;
-    const int stage = (kBlockM + p.N) * kLiChunk, other = 1024 + kLiCtrl + (p.splits > 1 ? p.N * kBlockM * 4 : 0);
+    const int b_rows = p.pair ? p.N / 2 : p.N, stage = (kBlockM + b_rows) * kLiChunk, other = 1024 + kLiCtrl + (p.splits > 1 ? p.N * kBlockM * 4 : 0);
     p.stages = std::min({kLiMaxStages, (kLiSmem - other) / stage, std::max(2, p.splits > 1 ? cdiv(p.chunks, p.splits) : kLiMaxStages)});
     p.spin_limit = wait_limit();
     p.drop_load = take_drop_load();
     CUtensorMap mapA, mapB;
     const void *A = nchw ? Q : W, *Bop = nchw ? W : Q;
     const long long lda = nchw ? ldq : ldw, ldb = nchw ? ldw : ldq;
-    if (!make_map_codes(&mapA, A, C, p.lanes, lda, kBlockM) || !make_map_codes(&mapB, Bop, C, p.cols, ldb, p.N)) return WG2X2_ERR_LAUNCH;
+    if (!make_map_codes(&mapA, A, C, p.lanes, lda, kBlockM) || !make_map_codes(&mapB, Bop, C, p.cols, ldb, b_rows)) return WG2X2_ERR_LAUNCH;
     const size_t smem = (size_t)other + (size_t)p.stages * stage;
-    if (type == WG2X2_F32) return nchw ? li_launch<true, float>(mapA, mapB, p, smem, st) : li_launch<false, float>(mapA, mapB, p, smem, st);
-    if (type == WG2X2_F16) return nchw ? li_launch<true, __half>(mapA, mapB, p, smem, st) : li_launch<false, __half>(mapA, mapB, p, smem, st);
-    return nchw ? li_launch<true, __nv_bfloat16>(mapA, mapB, p, smem, st) : li_launch<false, __nv_bfloat16>(mapA, mapB, p, smem, st);
+    if (type == WG2X2_F32) return nchw ? li_launch<true, float>(mapA, mapB, p, pairs, smem, st) : li_launch<false, float>(mapA, mapB, p, pairs, smem, st);
+    if (type == WG2X2_F16) return nchw ? li_launch<true, __half>(mapA, mapB, p, pairs, smem, st) : li_launch<false, __half>(mapA, mapB, p, pairs, smem, st);
+    return nchw ? li_launch<true, __nv_bfloat16>(mapA, mapB, p, pairs, smem, st) : li_launch<false, __nv_bfloat16>(mapA, mapB, p, pairs, smem, st);
 }

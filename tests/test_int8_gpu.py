@@ -236,7 +236,9 @@ def _check_linear(y, want, p, dtype):
 
 LINEAR = [(1, 1, 1), (1, 16, 3), (2, 17, 129), (3, 100, 64), (5, 128, 128), (7, 129, 1000), (16, 512, 1000), (17, 1000, 31), (31, 64, 257), (33, 127, 300), (64, 2048, 100),
           (100, 300, 513), (127, 4096, 128), (128, 128, 4100), (129, 1023, 255), (200, 40, 2048), (256, 512, 1000), (300, 8192, 70), (500, 384, 384), (1000, 256, 640),
-          (1111, 33, 777), (2049, 1100, 300), (5000, 64, 64), (3, 4096, 4096), (20000, 96, 24), (1, 5000, 20001), (40, 2000, 19000)]
+          (1111, 33, 777), (2049, 1100, 300), (5000, 64, 64), (3, 4096, 4096), (20000, 96, 24), (1, 5000, 20001), (40, 2000, 19000),
+          # tiles of 256 x 256 and 256 x 128 on pairs of SMs, ragged
+          (4100, 700, 3001), (3000, 1024, 2048), (8192, 300, 4097), (2600, 2000, 5000), (700, 4100, 9000)]
 
 
 @pytest.mark.parametrize("rows,C,K", LINEAR)
@@ -256,7 +258,7 @@ def test_linear(rows, C, K):
 
 
 @pytest.mark.parametrize("B,H,W,C,K", [(1, 1, 1, 5, 3), (1, 7, 7, 512, 100), (2, 7, 7, 64, 64), (3, 5, 9, 130, 33), (4, 28, 28, 64, 128), (1, 56, 56, 64, 64), (40, 14, 14, 128, 256),
-                                       (64, 7, 7, 256, 512), (2, 1, 130, 2000, 17), (30, 28, 27, 33, 300)])
+                                       (64, 7, 7, 256, 512), (2, 1, 130, 2000, 17), (30, 28, 27, 33, 300), (64, 14, 14, 600, 1030), (17, 28, 28, 1024, 513)])
 def test_linear_images(B, H, W, C, K):
     g = _gen("li", B, H, W, C, K)
     rows = B * H * W
