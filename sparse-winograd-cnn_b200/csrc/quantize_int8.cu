@@ -222,9 +222,8 @@ __device__ __noinline__ unsigned near_tie(float u, float inv, float a)
 // also the one nearest to 127 u / a; elsewhere near_tie says (u = a / 2 is common in 16-bit types, and there are rows with a tie in every
 // dozen values).  a below kTinyRow or not finite: inv = 0, and the caller clears the codes.
 template <int N>
-__device__ __forceinline__ void code_words(const float (&u)[N], float inv, float a, unsigned (&w)[N / 4])
+__device__ __forceinline__ float fast_codes(const float (&u)[N], float inv, unsigned (&w)[N / 4], float off = 0.f)      // -> the largest |d|
 {
-    float off = 0.f;
 #pragma unroll
     for (int g = 0; g < N / 4; ++g) {
         unsigned r[4];
@@ -236,14 +235,22 @@ __device__ __forceinline__ void code_words(const float (&u)[N], float inv, float
         }
         w[g] = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
     }
-    if (off > kNearTie) {
+    return off;
+}
+template <int N>
+__device__ __forceinline__ void mend_codes(const float (&u)[N], float inv, float a, unsigned (&w)[N / 4])
+{
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float x = u[j], m = fmaf(x, inv, kRound);
-            if (fabsf(fmaf(x, inv, -__fsub_rn(m, kRound))) > kNearTie)
-                w[j / 4] = __byte_perm(w[j / 4], near_tie(x, inv, a), (j & 3) == 0 ? 0x3214 : (j & 3) == 1 ? 0x3240 : (j & 3) == 2 ? 0x3410 : 0x4210);
-        }
+    for (int j = 0; j < N; ++j) {
+        const float x = u[j], m = fmaf(x, inv, kRound);
+        if (fabsf(fmaf(x, inv, -__fsub_rn(m, kRound))) > kNearTie)
+            w[j / 4] = __byte_perm(w[j / 4], near_tie(x, inv, a), (j & 3) == 0 ? 0x3214 : (j & 3) == 1 ? 0x3240 : (j & 3) == 2 ? 0x3410 : 0x4210);
     }
+}
+template <int N>
+__device__ __forceinline__ void code_words(const float (&u)[N], float inv, float a, unsigned (&w)[N / 4])
+{
+    if (fast_codes<N>(u, inv, w) > kNearTie) mend_codes<N>(u, inv, a, w);
 }
 
 struct RowCodes {
@@ -312,7 +319,7 @@ __device__ __forceinline__ void reduce_block(float &a, float &ss, float2 *part)
 // boundary in every row.  The aligned pieces that a row touches come to shared memory; there the shortcut is added to them, and every
 // thread then reads its N channels at the offset that the row has.
 template <typename T, int MODE, int V, bool BLOCK, bool ODD, int AHEAD>
-__global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256) rows_kernel(const RowsParams p)
+__global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256, !BLOCK && V == 4 ? 3 : 1) rows_kernel(const RowsParams p)
 {
     constexpr int N = 16 / sizeof(T), WORDS = N / 4, STAGES = AHEAD + 1;
     constexpr bool SUM = MODE != kQuantize;
@@ -564,10 +571,10 @@ __global__ void __launch_bounds__(512) rows_any_kernel(const RowsParams p)
 // NCHW: lane = pixel (of any images), so that a load is 32 consecutive values of a plane.  p.group warps share a tile of 32 pixels, each
 // with groups of four neighbouring channels, whose codes are a word: NQ groups a thread (0: any number, read a second time).  As many as
 // registers allow, because a thread has costs of its own per pixel (its image, the divisions, the meeting of its warps).  The words are turned through shared memory and leave as pieces of rows.
-template <typename T, int MODE, int NQ>
+template <typename T, int MODE, int NQ, bool FULL>
 __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
 {
-    extern __shared__ unsigned turned_all[];        // [tile of the block][32][pitch]
+    extern __shared__ unsigned turned_all[];        // [tile of the block][32][pitch], then the weights
     __shared__ float2 part[2][16][32];
     constexpr bool SUM = MODE != kQuantize;
     wait_for_previous_kernel(kNumSMs);
@@ -575,75 +582,90 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
     const int tile = warp / share, wi = warp - tile * share, tiles = (blockDim.x >> 5) / share;
     const long long row0 = ((long long)blockIdx.x * tiles + tile) * 32, row = row0 + lane;
     const bool have = row < p.rows;
-    long long base = 0;
-    if (have) {
-        if (p.rows <= 0x7fffffffLL) {
-            const unsigned b = (unsigned)row / (unsigned)p.HW;
-            base = (long long)b * p.C * p.HW + ((unsigned)row - b * (unsigned)p.HW);
-        } else {
-            const long long b = row / p.HW;
-            base = b * p.C * p.HW + (row - b * p.HW);
-        }
+    const long long src = have ? row : p.rows - 1;          // (a lane without a pixel reads the last one, and stores nothing)
+    long long base;
+    if (p.rows <= 0x7fffffffLL) {
+        const unsigned b = (unsigned)src / (unsigned)p.HW;
+        base = (long long)b * p.C * p.HW + ((unsigned)src - b * (unsigned)p.HW);
+    } else {
+        const long long b = src / p.HW;
+        base = b * p.C * p.HW + (src - b * p.HW);
     }
     const T *x = static_cast<const T *>(p.X) + base;
     const T *res = MODE == kNormRes ? static_cast<const T *>(p.R) + base : nullptr;
     T *h = MODE == kNormRes ? static_cast<T *>(p.H) + base : nullptr;
-    const int words = (p.C + 3) >> 2, pitch = words | 1, C = have ? p.C : 0;
-    const unsigned HW = p.HW;                       // (a channel's offset in its image fits 31 bits, but for NQ = 0)
+    const int C = p.C, words = (C + 3) >> 2, pitch = words | 1;
+    const long long HW = p.HW;
     const float low = p.relu ? 0.f : __uint_as_float(0xff800000u);
     auto value = [&](float v, int c) { return MODE != kQuantize ? __fmul_rn(v, weight_at(p, (const T *)nullptr, c)) : at_least(v, low); };
+    float *weights = reinterpret_cast<float *>(turned_all) + tiles * 32 * pitch;
+    if (NQ && SUM) {
+        for (int c = threadIdx.x; c < 4 * words; c += blockDim.x) weights[c] = c < C ? weight_at(p, (const T *)nullptr, c) : 0.f;
+        __syncthreads();
+    }
 
     constexpr int KEEP = NQ ? NQ : 1;
     float u[KEEP][4];
     float amax = 0.f, ss = 0.f;
     if (NQ) {
+        // the thread's groups of four channels: wi, wi + share, ...; FULL: all of them exist, with all four
+        const long long step = 4 * share * HW, at0 = 4 * wi * HW;
+        auto load = [&](const T *t, float (&v)[4], int g) {
+            if (FULL) {
 #pragma unroll
-        for (int g = 0; g < KEEP; ++g)
+                for (int j = 0; j < 4; ++j) v[j] = to_f(t[j * HW]);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const unsigned c = 4 * (wi + g * share) + j;
-                u[g][j] = c < (unsigned)C ? to_f(x[c * HW]) : 0.f;
+                for (int j = 0; j < 4; ++j) v[j] = 4 * (wi + g * share) + j < C ? to_f(t[j * HW]) : 0.f;
             }
+        };
+        const T *t = x + at0;
+#pragma unroll
+        for (int g = 0; g < KEEP; ++g, t += step) load(t, u[g], g);
         if (MODE == kNormRes) {
             constexpr int HALF = KEEP > 8 ? 8 : KEEP;
+            const T *t = res + at0;
+            T *o = h + at0;
 #pragma unroll
             for (int g0 = 0; g0 < KEEP; g0 += HALF) {
                 float r[HALF][4];
 #pragma unroll
-                for (int g = 0; g < HALF; ++g)
+                for (int g = 0; g < HALF; ++g, t += step) load(t, r[g], g0 + g);
+#pragma unroll
+                for (int g = 0; g < HALF; ++g, o += step)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const unsigned c = 4 * (wi + (g0 + g) * share) + j;
-                        r[g][j] = c < (unsigned)C ? to_f(res[c * HW]) : 0.f;
-                    }
-#pragma unroll
-                for (int g = 0; g < HALF; ++g)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const unsigned c = 4 * (wi + (g0 + g) * share) + j;
                         const T s = from_f<T>(__fadd_rn(u[g0 + g][j], r[g][j]));
-                        if (c < (unsigned)C) h[c * HW] = s;
+                        if (have && (FULL || 4 * (wi + (g0 + g) * share) + j < C)) o[j * HW] = s;
                         u[g0 + g][j] = to_f(s);
                     }
             }
         }
 #pragma unroll
         for (int g = 0; g < KEEP; ++g) {
+            if (SUM) {
+                const int q = wi + g * share;
+                const float4 w4 = FULL || q < words ? *reinterpret_cast<const float4 *>(weights + 4 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = 4 * (wi + g * share) + j;
-                if (SUM) ss = fmaf(u[g][j], u[g][j], ss);
-                u[g][j] = MODE != kQuantize && c >= p.C ? 0.f : value(u[g][j], c);
-                amax = mag_max(amax, u[g][j]);
+                for (int j = 0; j < 4; ++j) {
+                    ss = fmaf(u[g][j], u[g][j], ss);
+                    u[g][j] = __fmul_rn(u[g][j], w[j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[g][j] = at_least(u[g][j], low);
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) amax = mag_max(amax, u[g][j]);
         }
     } else {
         for (int c = wi; c < C; c += share) {
-            const long long o = (long long)c * HW;
+            const long long o = c * HW;
             float v = to_f(x[o]);
             if (MODE == kNormRes) {
                 const T s = from_f<T>(__fadd_rn(v, to_f(res[o])));
-                h[o] = s;
+                if (have) h[o] = s;
                 v = to_f(s);
             }
             ss = fmaf(v, v, ss);
@@ -671,7 +693,7 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
             const T *again = MODE == kNormRes ? h : x;          // (h as any of these warps stored it: there has been a barrier)
             float s2 = 0.f, none = 0.f;
             for (int c = wi; c < C; c += share) {
-                const float f = to_f(again[(long long)c * HW]) * kDown;
+                const float f = to_f(again[c * HW]) * kDown;
                 s2 = fmaf(f, f, s2);
             }
             over_warps(none, s2, 1);
@@ -683,12 +705,18 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
     }
     if (NQ) {
         unsigned *turned = turned_all + tile * 32 * pitch;
+        unsigned w[KEEP][1];
+        float off = 0.f;
+#pragma unroll
+        for (int g = 0; g < KEEP; ++g) off = fast_codes<4>(u[g], k.inv, w[g], off);
+        if (off > kNearTie) {
+#pragma unroll
+            for (int g = 0; g < KEEP; ++g) mend_codes<4>(u[g], k.inv, k.a, w[g]);
+        }
 #pragma unroll
         for (int g = 0; g < KEEP; ++g) {
             const int q = wi + g * share;
-            unsigned w[1];
-            code_words<4>(u[g], k.inv, k.a, w);
-            if (q < words) turned[lane * pitch + q] = w[0] & k.live;
+            if (FULL || q < words) turned[lane * pitch + q] = w[g][0] & k.live;
         }
         if (share == 1) __syncwarp();
         else __syncthreads();
@@ -715,12 +743,12 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
         }
     } else {
         // (h as any warp stored it: over_warps is a barrier)
-        for (int q = wi; 4 * q < C; q += share) {
+        for (int q = wi; have && 4 * q < C; q += share) {
             float v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int c = 4 * q + j;
-                v[j] = c < p.C ? value(to_f((MODE == kNormRes ? h : x)[(long long)c * HW]), c) : 0.f;
+                v[j] = c < C ? value(to_f((MODE == kNormRes ? h : x)[c * HW]), c) : 0.f;
             }
             unsigned codes[1];
             code_words<4>(v, k.inv, k.a, codes);
@@ -728,7 +756,7 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
             signed char *dst = p.Q + row * p.ldq + 4 * q;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (4 * q + j < p.C) dst[j] = (signed char)(w >> (8 * j));
+                if (4 * q + j < C) dst[j] = (signed char)(w >> (8 * j));
         }
     }
 }
@@ -795,7 +823,7 @@ static int rows_int8(RowsParams p, cudaStream_t st)
 template <typename T, int MODE>
 static int nchw_int8(RowsParams p, cudaStream_t st)
 {
-    const int words = cdiv(p.C, 4); const int most = words <= 128 ? 8 : 16;
+    const int words = cdiv(p.C, 4), most = MODE == kNormRes && words <= 128 ? 8 : 16;
     const long long tiles = cdivll(p.rows, 32);
     // warps that share 32 pixels: as few as the registers allow, more where the pixels are few
     int share = 1;
@@ -804,19 +832,20 @@ static int nchw_int8(RowsParams p, cudaStream_t st)
     const bool loop = words > share * most || (long long)p.C * p.HW > 0x7fffffffLL;
     if (loop) share = 16;
     p.group = share;
-    const int warps = std::max(8, share), per_block = warps / share;
+    const int warps = std::max(2, share), per_block = warps / share;
     const long long blocks = cdivll(tiles, per_block);
     if (blocks > 0x7fffffffLL) return WG2X2_ERR_UNSUPPORTED;
     const bool by16 = p.C % 16 == 0 && p.ldq % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Q) & 15u) == 0;
     const int pieces = by16 ? words / 4 : words;
     p.inv = pieces > 1 ? (unsigned)((0x100000000ull + pieces - 1) / pieces) : 0;       // i / pieces exact for i * pieces < 2^32
-    const size_t smem = (size_t)per_block * 32 * (words | 1) * 4;
-    const int nq = cdiv(words, share);
-    if (loop) return launch(nchw_kernel<T, MODE, 0>, dim3((unsigned)blocks), 32 * warps, 0, st, p);
-    if (nq <= 2) return launch(nchw_kernel<T, MODE, 2>, dim3((unsigned)blocks), 32 * warps, smem, st, p);
-    if (nq <= 4) return launch(nchw_kernel<T, MODE, 4>, dim3((unsigned)blocks), 32 * warps, smem, st, p);
-    if (nq <= 8) return launch(nchw_kernel<T, MODE, 8>, dim3((unsigned)blocks), 32 * warps, smem, st, p);
-    return launch(nchw_kernel<T, MODE, 16>, dim3((unsigned)blocks), 32 * warps, smem, st, p);
+    const size_t smem = loop ? 0 : (size_t)per_block * 32 * (words | 1) * 4 + (MODE != kQuantize ? (size_t)16 * words : 0);
+    const int nq = loop ? 0 : cdiv(words, share) <= 2 ? 2 : cdiv(words, share) <= 4 ? 4 : cdiv(words, share) <= 8 ? 8 : 16;
+    const bool full = p.C == 4 * nq * share;
+#define WG_NCHW(NQ)                                                                                                          \
+    (full ? launch(nchw_kernel<T, MODE, NQ, (NQ) != 0>, dim3((unsigned)blocks), 32 * warps, smem, st, p)                      \
+          : launch(nchw_kernel<T, MODE, NQ, false>, dim3((unsigned)blocks), 32 * warps, smem, st, p))
+    return nq == 0 ? WG_NCHW(0) : nq == 2 ? WG_NCHW(2) : nq == 4 ? WG_NCHW(4) : nq == 8 ? WG_NCHW(8) : WG_NCHW(16);
+#undef WG_NCHW
 }
 
 static int codes_int8(int mode, int type, RowsParams &p, long long B, int HW, int C, int layout, cudaStream_t st)
