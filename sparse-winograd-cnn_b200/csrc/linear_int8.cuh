@@ -263,12 +263,32 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
     volatile int *abort_flag = reinterpret_cast<volatile int *>(ctrl_gen + 8 * (2 * kLiMaxStages + 5));
     static_assert(8 * (2 * kLiMaxStages + 6) <= 512, "control block");
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int rank = SPLIT ? (int)cluster_ctarank() : 0;
+    const int first = SPLIT ? blockIdx.x / prm.splits : blockIdx.x, step = SPLIT ? 1 << 30 : (int)gridDim.x;
+    const int units = prm.lane_tiles * prm.col_tiles;
+    // (at least one chunk for every CTA: splits <= chunks)
+    const int kbeg = SPLIT ? rank * prm.chunks / prm.splits : 0, kend = SPLIT ? (rank + 1) * prm.chunks / prm.splits : prm.chunks;
+    auto load = [&](int s, int lt, int ct, int kc) {
+        mbar_expect_tx(full_bar(s), (uint32_t)stage_bytes);
+        const uint32_t dst = base + s * stage_bytes;
+        tma_load_2d(dst, &mapA, full_bar(s), kc * kLiChunk, lt * kBlockM);
+        tma_load_2d(dst + kBlockM * kLiChunk, &mapB, full_bar(s), kc * kLiChunk, ct * prm.N);
+    };
+    // The first tile's loads, as many as there are stages, go out before the rest of the set-up
+    if (threadIdx.x == 32 || threadIdx.x == 64)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(threadIdx.x == 32 ? &mapA : &mapB) : "memory");
+    const int early = prm.drop_load >= 0 ? 0 : min(prm.stages, kend - kbeg);
     if (threadIdx.x == 0) {
         for (int s = 0; s < prm.stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), kLiEpiWarps); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        int lt, ct;
+        li_decode(prm, first, lt, ct);
+        wait_for_previous_kernel(kNumSMs);
+        for (int s = 0; s < early; ++s) load(s, lt, ct, kbeg + s);
     }
+    __syncwarp();
     if (warp == 1) {
         tmem_alloc(smem_u32((const void *)tmem_ptr_slot), kTmemCols);
         tmem_relinquish();
@@ -278,30 +298,25 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
     if (SPLIT) cluster_sync_all();                  // (a CTA's shared memory is written by others only once it runs)
     tc_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_slot, 0);
-    wait_for_previous_kernel(kNumSMs);
-
-    const int rank = SPLIT ? (int)cluster_ctarank() : 0;
-    const int first = SPLIT ? blockIdx.x / prm.splits : blockIdx.x, step = SPLIT ? 1 << 30 : (int)gridDim.x;
-    const int units = prm.lane_tiles * prm.col_tiles;
-    // (at least one chunk for every CTA: splits <= chunks)
-    const int kbeg = SPLIT ? rank * prm.chunks / prm.splits : 0, kend = SPLIT ? (rank + 1) * prm.chunks / prm.splits : prm.chunks;
+    if (threadIdx.x != 0) wait_for_previous_kernel(kNumSMs);
     bool ok = true;
+    // SPLIT: an epilogue thread's lane of the tile, and of its columns (part, part + 4, ... of the CTA's) the lane-th; asked for while the
+    // products run
+    int lt, ct;
+    LiScale lane_scale = {};
+    float col_scale = 0.f, col_bias = -0.f;
 
     if (warp == 0) {
         if (lane == 0) {
-            int s = 0, loads = 0;
-            uint32_t ph = 0;
-            const uint32_t bytes = (uint32_t)stage_bytes;
+            int s = early % prm.stages, loads = 0;
+            uint32_t ph = early == prm.stages ? 1 : 0;
             for (int u = first; u < units && ok; u += step) {
                 int lt, ct;
                 li_decode(prm, u, lt, ct);
-                for (int kc = kbeg; kc < kend; ++kc) {
+                for (int kc = kbeg + (u == first ? early : 0); kc < kend; ++kc) {
                     if (loads++ == prm.drop_load && blockIdx.x == 0) { ok = false; break; }
                     if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, 0x1C00u | s, prm.spin_limit)) { ok = false; break; }
-                    mbar_expect_tx(full_bar(s), bytes);
-                    const uint32_t dst = base + s * stage_bytes;
-                    tma_load_2d(dst, &mapA, full_bar(s), kc * kLiChunk, lt * kBlockM);
-                    tma_load_2d(dst + kBlockM * kLiChunk, &mapB, full_bar(s), kc * kLiChunk, ct * prm.N);
+                    load(s, lt, ct, kc);
                     if (++s == prm.stages) { s = 0; ph ^= 1u; }
                 }
                 if (step == 1 << 30) break;
@@ -347,6 +362,13 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
                                       [](uint32_t bar) { mbar_arrive(bar); });
         } else {
             // this CTA's share of the sums to the CTAs that finish them: [share][column][lane]
+            li_decode(prm, first, lt, ct);
+            lane_scale = li_lane_scale<NCHW>(prm, lt * kBlockM + q * 32 + lane);
+            const int c = part + 4 * lane, col = ct * prm.N + rank * (prm.N / prm.splits) + c;
+            if (c < prm.N / prm.splits && col < prm.cols) {
+                col_scale = prm.col_scale[col];
+                if (NCHW && prm.bias) col_bias = prm.bias[col];
+            }
             ok = mbar_wait_warp(accf_bar(0), 0, abort_flag, 0x1F00u, prm.spin_limit);
             tc_fence_after();
             if (ok) {
@@ -371,19 +393,16 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
         __syncwarp();
         cluster_sync_all();                         // every thread of every CTA, whatever came before
         if (warp >= 2) {
-            int lt, ct;
-            li_decode(prm, first, lt, ct);
             const int q = warp & 3, part = (warp - 2) >> 2, mine = prm.N / prm.splits;
-            const int lane_row = lt * kBlockM + q * 32 + lane;
-            const LiLane<NCHW, T> me(prm, lane_row, li_lane_scale<NCHW>(prm, lane_row));
+            const LiLane<NCHW, T> me(prm, lt * kBlockM + q * 32 + lane, lane_scale);
             const int *sums = reinterpret_cast<const int *>(ctrl_gen + kLiCtrl) + q * 32 + lane;
             for (int c = part; c < mine; c += 4) {
                 const int col = ct * prm.N + rank * mine + c;
                 if (col >= prm.cols) break;
                 int acc = 0;
                 for (int s = 0; s < prm.splits; ++s) acc += sums[(s * mine + c) * kBlockM];
-                const float cs = prm.col_scale[col], b = NCHW ? (prm.bias ? prm.bias[col] : -0.f) : me.bias;
-                const float v = NCHW ? li_value(acc, cs, me.scale, b, me.low) : li_value(acc, me.scale, cs, b, me.low);
+                const float cs = __shfl_sync(0xffffffffu, col_scale, c >> 2), cb = NCHW ? __shfl_sync(0xffffffffu, col_bias, c >> 2) : me.bias;
+                const float v = NCHW ? li_value(acc, cs, me.scale, cb, me.low) : li_value(acc, me.scale, cs, cb, me.low);
                 if (me.live) me.dst[col * me.step] = li_out<T>(v);
             }
         }
@@ -519,6 +538,87 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_c
     }
 }
 
+// A few rows of codes: nothing but the weights' bytes counts, and the set-up of the kernels above (tensor memory, barriers, a cluster's
+// exchange) would take longer than those.  `group` lanes have a row of weights, 16 bytes a load and eight loads on their way, and multiply
+// four codes an instruction.
+constexpr int kLiFewRows = 4;
+struct LiFewParams {
+    const signed char *Q, *W;
+    const float *q_scale, *w_scale, *bias;
+    void *Y;
+    long long ldq, ldw, ldy;
+    int rows, C, K, HW, group, relu;        // HW: 0, or an NCHW result's pixels
+};
+// (NR rows of weights at a time where there are several rows of codes, so that a load of those serves as many products)
+template <int ROWS, int NR, typename T>
+__global__ void __launch_bounds__(128) linear_int8_few_kernel(const LiFewParams p)
+{
+    constexpr int AT_ONCE = 8 / NR;
+    wait_for_previous_kernel(8 * kNumSMs);
+    const int at = threadIdx.x & (p.group - 1), k = (int)(((long long)blockIdx.x * 128 + threadIdx.x) / p.group) * NR;
+    const signed char *w[NR], *q[ROWS];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) w[n] = p.W + min(k + n, p.K - 1) * p.ldw;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) q[r] = p.Q + min(r, p.rows - 1) * p.ldq;
+    int acc[NR][ROWS];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) acc[n][r] = 0;
+    const int pieces = p.C >> 4;
+    for (int i0 = at; i0 < pieces; i0 += AT_ONCE * p.group) {
+        int4 v[AT_ONCE][NR];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int i = i0 + j * p.group;
+#pragma unroll
+            for (int n = 0; n < NR; ++n) v[j][n] = i < pieces ? *reinterpret_cast<const int4 *>(w[n] + 16LL * i) : make_int4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int i = min(i0 + j * p.group, pieces - 1);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const int4 x = *reinterpret_cast<const int4 *>(q[r] + 16LL * i);
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+                    acc[n][r] = __dp4a(v[j][n].x, x.x, __dp4a(v[j][n].y, x.y, __dp4a(v[j][n].z, x.z, __dp4a(v[j][n].w, x.w, acc[n][r]))));
+            }
+        }
+    }
+    for (int c = 16 * pieces + at; c < p.C; c += p.group)
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) acc[n][r] += (int)w[n][c] * (int)q[r][c];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            for (int o = p.group >> 1; o; o >>= 1) acc[n][r] += __shfl_xor_sync(0xffffffffu, acc[n][r], o);
+    if (at) return;
+    const float low = p.relu ? 0.f : __uint_as_float(0xff800000u);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        if (k + n >= p.K) break;
+        const float ws = p.w_scale[k + n], b = p.bias ? p.bias[k + n] : -0.f;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            if (r >= p.rows) break;
+            const long long to = p.HW ? (long long)(r / p.HW) * p.K * p.HW + r % p.HW + (long long)(k + n) * p.HW : r * p.ldy + k + n;
+            static_cast<T *>(p.Y)[to] = li_out<T>(li_value(acc[n][r], ws, p.q_scale[r], b, low));
+        }
+    }
+}
+template <typename T>
+static int li_few(LiFewParams p, cudaStream_t st)
+{
+    for (p.group = 4; p.group < 32 && p.group * 16 < p.C;) p.group *= 2;
+    auto *kernel = p.rows == 1 ? linear_int8_few_kernel<1, 1, T> : p.rows == 2 ? linear_int8_few_kernel<2, 2, T> : linear_int8_few_kernel<4, 2, T>;
+    return launch(kernel, dim3((unsigned)cdivll(p.K, 128 / p.group * (p.rows == 1 ? 1 : 2))), 128, 0, st, p);
+}
+
 // ---------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------
@@ -538,44 +638,63 @@ static bool make_map_codes(CUtensorMap *map, const void *ptr, int C, long long r
     return r == CUDA_SUCCESS;
 }
 
-// Pairs of SMs that run at once
-static int li_pairs()
+// Clusters of 2, 4 and 8 CTAs that run at once ([1], [2], [3]; of kernels that need a whole SM)
+struct LiClusters { int n[4]; };
+static LiClusters li_clusters()
 {
-    static std::atomic<int> known[64];           // 0: not asked yet, else the number + 1
+    static std::atomic<unsigned long long> known[64];           // 0: not asked yet, else 1 and the three numbers, 16 bits each
+    LiClusters c = {};
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    int n = known[dev].load();
-    if (n) return n - 1;
-    auto *kernel = linear_int8_pair_kernel<false, float>;
-    if (grant_smem(reinterpret_cast<const void *>(kernel), kLiSmem)) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(kNumSMs);
-        cfg.blockDim = dim3(kLiThreads);
-        cfg.dynamicSmemBytes = kLiSmem;
-        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { n = 0; (void)cudaGetLastError(); }
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return c;
+    unsigned long long v = known[dev].load();
+    if (!v) {
+        v = 1;
+        auto *kernel = linear_int8_kernel<false, float, true>;
+        for (int i = 1; i < 4 && grant_smem(reinterpret_cast<const void *>(kernel), kLiSmem); ++i) {
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1u << i;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(8 * kNumSMs);
+            cfg.blockDim = dim3(kLiThreads);
+            cfg.dynamicSmemBytes = kLiSmem;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { n = 0; (void)cudaGetLastError(); }
+            v |= (unsigned long long)(n & 0xffff) << (16 * i);
+        }
+        known[dev].store(v);
     }
-    known[dev].store(n + 1);
-    return n;
+    for (int i = 1; i < 4; ++i) c.n[i] = (int)((v >> (16 * i)) & 0xffff);
+    return c;
 }
 
-// Columns of a tile, CTAs that share one, and whether pairs of SMs do, by an estimate in clocks: a chunk of operands comes from L2 at about
-// 64 bytes a clock and SM, the tensor cores take 2 clocks for a chunk of a column; a column of 128 lanes is finished in about 10 clocks and
-// a tile in 600 more (beside the next tile's products, where there is one); a shared tile costs a cluster's barrier and exchange.
-static void li_choose(LiParams &p, int pairs)
+// Columns of a tile, CTAs that share one, and whether pairs of SMs do, by an estimate in clocks.  Operands reach an SM at 55 bytes a
+// clock, one of a pair at 42, all SMs together at 6500 (3400 from memory): more than the products themselves take.  A column of 128 lanes is finished in about 10 clocks and a tile in 600 more, beside the next tile's products where there is one.  CTAs that share a
+// tile: two cluster barriers, and the sums' way between SMs, which is narrow.  Measured in a graph, us, C x K x rows, (N, S) taken / next
+// best / a worse one: 2048 x 8191 x 24 (32, 1) 6.4 / (16, 1) 7.0 / (32, 2) 8.0; 4096 x 4096 x 16 (16, 4) 7.0 / (16, 2) 8.4 / (16, 1) 9.1;
+// 4096 x 4096 x 256 (64, 1) 10.4 / (128, 1) 11.3 / (128, 2) 14.8; 8192 x 1024 x 100 (32, 4) 9.5 / (128, 8) 9.8 / (64, 8) 16.4.
+static void li_choose(LiParams &p, const LiClusters &clusters)
 {
     double best = 1e300;
     const int lanes = p.lanes;
+    const double from_memory = 128.0 * p.chunks * ((double)lanes + p.cols) / 3400;
     for (int N = 16; N <= 256; N *= 2) {
         const long long cols = cdiv(p.cols, N), tiles = cols * cdiv(lanes, kBlockM);
-        for (int S = 1; S <= 8; S *= 2) {
-            if (S > 1 && (N > 128 || S > p.chunks || tiles * S > kNumSMs)) break;
-            const double main = (double)cdiv(p.chunks, S) * 2 * (kBlockM + N), store = (600 + 10.0 * N) / S;
-            const double t = (double)cdivll(tiles * S, kNumSMs) * std::max(main, store) + std::min(main, store) + (S > 1 ? 1000 + 4 * N : 0);
+        const double bytes = std::max(from_memory, 128.0 * p.chunks * (double)tiles * (kBlockM + N) / 6500), column = 600 + 10.0 * N;
+        for (int i = 0; i < 4; ++i) {
+            const int S = 1 << i;
+            if (S > 1 && (N > 128 || S > p.chunks || tiles > clusters.n[i])) break;
+            const double main = (double)cdiv(p.chunks, S) * 128 * (kBlockM + N) / 55, store = column / S;
+            const double t = std::max(bytes, (double)cdivll(tiles * S, kNumSMs) * std::max(main, store)) + std::min(main, store) + (S > 1 ? 1500 + 90 * N : 0);
             if (t < best * 0.999) { best = t; p.N = N; p.splits = S; p.pair = 0; }
         }
-        if (N >= 128 && pairs > 0) {
-            const double main = (double)p.chunks * std::max(2 * N, 256 + N), store = 600 + 10.0 * N;
-            const double t = (double)cdivll(cols * cdiv(lanes, 256), pairs) * std::max(main, store) + std::min(main, store) + 500;
+        if (N >= 128 && clusters.n[1] > 0) {
+            const long long pairs = cols * cdiv(lanes, 256);
+            const double main = (double)p.chunks * 128 * (kBlockM + N / 2) / 42, two = std::max(from_memory, 128.0 * p.chunks * (double)pairs * (256 + N) / 6500);
+            const double t = std::max(two, (double)cdivll(pairs, clusters.n[1]) * std::max(main, column)) + std::min(main, column) + 1500;
             if (t < best * 0.999) { best = t; p.N = N; p.splits = 1; p.pair = 1; }
         }
     }
@@ -615,6 +734,13 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     auto meets = [&](const void *p, long long ld, long long n, long long count) { return p && rows_overlap(Y, ypitch, ybytes, ny, p, ld, n, count); };
     if (meets(Q, ldq, C, rows) || meets(W, ldw, C, K) || meets(q_scale, 0, 4 * rows, 1) || meets(w_scale, 0, 4LL * K, 1) || meets(bias, 0, 4LL * K, 1))
         return WG2X2_ERR_BAD_ARG;
+    if (rows <= kLiFewRows) {
+        LiFewParams f = {};
+        f.Q = static_cast<const signed char *>(Q); f.W = static_cast<const signed char *>(W);
+        f.q_scale = q_scale; f.w_scale = w_scale; f.bias = bias; f.Y = Y; f.ldq = ldq; f.ldw = ldw; f.ldy = ldy;
+        f.rows = (int)rows; f.C = C; f.K = K; f.HW = nchw ? HW : 0; f.relu = relu != 0;
+        return type == WG2X2_F32 ? li_few<float>(f, st) : type == WG2X2_F16 ? li_few<__half>(f, st) : li_few<__nv_bfloat16>(f, st);
+    }
     LiParams p = {};
     p.Y = Y; p.ldy = ldy; p.bias = bias; p.K = K; p.HW = HW; p.relu = relu != 0;
     p.lane_scale = nchw ? q_scale : w_scale;
@@ -622,8 +748,9 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     p.lanes = nchw ? (int)rows : K;
     p.cols = nchw ? K : (int)rows;
     p.chunks = cdiv(C, kLiChunk);
-    const int pairs = li_pairs();
-    li_choose(p, pairs);
+    const LiClusters clusters = li_clusters();
+    li_choose(p, clusters);
+    const int pairs = clusters.n[1];
     if ((long long)p.lane_tiles * p.col_tiles > 0x3fffffffLL) return WG2X2_ERR_UNSUPPORTED;
     const int b_rows = p.pair ? p.N / 2 : p.N, stage = (kBlockM + b_rows) * kLiChunk, other = 1024 + kLiCtrl + (p.splits > 1 ? p.N * kBlockM * 4 : 0);
     p.stages = std::min({kLiMaxStages, (kLiSmem - other) / stage, std::max(2, p.splits > 1 ? cdiv(p.chunks, p.splits) : kLiMaxStages)});

@@ -234,7 +234,7 @@ def _check_linear(y, want, p, dtype):
     assert bool((y.double().abs() >= torch.finfo(dtype).max)[big].all())
 
 
-LINEAR = [(1, 1, 1), (1, 16, 3), (2, 17, 129), (3, 100, 64), (5, 128, 128), (7, 129, 1000), (16, 512, 1000), (17, 1000, 31), (31, 64, 257), (33, 127, 300), (64, 2048, 100),
+LINEAR = [(1, 1, 1), (4, 15, 9), (4, 31, 100), (2, 500, 700), (3, 129, 33), (4, 4096, 4096), (1, 9000, 300), (1, 16, 3), (2, 17, 129), (3, 100, 64), (5, 128, 128), (7, 129, 1000), (16, 512, 1000), (17, 1000, 31), (31, 64, 257), (33, 127, 300), (64, 2048, 100),
           (100, 300, 513), (127, 4096, 128), (128, 128, 4100), (129, 1023, 255), (200, 40, 2048), (256, 512, 1000), (300, 8192, 70), (500, 384, 384), (1000, 256, 640),
           (1111, 33, 777), (2049, 1100, 300), (5000, 64, 64), (3, 4096, 4096), (20000, 96, 24), (1, 5000, 20001), (40, 2000, 19000),
           # tiles of 256 x 256 and 256 x 128 on pairs of SMs, ragged
@@ -257,7 +257,7 @@ def test_linear(rows, C, K):
         _check_linear(y, want, p, dtype)
 
 
-@pytest.mark.parametrize("B,H,W,C,K", [(1, 1, 1, 5, 3), (1, 7, 7, 512, 100), (2, 7, 7, 64, 64), (3, 5, 9, 130, 33), (4, 28, 28, 64, 128), (1, 56, 56, 64, 64), (40, 14, 14, 128, 256),
+@pytest.mark.parametrize("B,H,W,C,K", [(1, 1, 1, 5, 3), (2, 1, 2, 100, 7), (1, 1, 3, 512, 1000), (1, 7, 7, 512, 100), (2, 7, 7, 64, 64), (3, 5, 9, 130, 33), (4, 28, 28, 64, 128), (1, 56, 56, 64, 64), (40, 14, 14, 128, 256),
                                        (64, 7, 7, 256, 512), (2, 1, 130, 2000, 17), (30, 28, 27, 33, 300), (64, 14, 14, 600, 1030), (17, 28, 28, 1024, 513)])
 def test_linear_images(B, H, W, C, K):
     g = _gen("li", B, H, W, C, K)
@@ -425,7 +425,7 @@ def test_streams_threads_and_graphs():
     assert not bad
 
 
-@pytest.mark.parametrize("rows,C,K", [(4, 4096, 256), (3000, 256, 1024)])
+@pytest.mark.parametrize("rows,C,K", [(9, 4096, 256), (3000, 256, 1024), (6000, 1024, 4096)])
 def test_time_out_of_the_product(rows, C, K):
     """A load that never comes: the wait for it gives up, the status says so, and the next call is right"""
     from wg2x2._lib import lib
