@@ -8,7 +8,8 @@ after a ReLU.  The reference has `pool4` commented out (:191), so its stage 5 ru
 `stage5_pool=True` restores the pool (7x7), which is the shape the benchmark configuration names.
 
 The Winograd layers and, for NCHW activations, the stem, the pools and the 1x1 shortcuts of few pixels run on this repository's
-kernels; the other 1x1 shortcuts and the classifier are stock torch ops.  With layout="NCHW" the layers of the two high-resolution
+kernels; the other 1x1 shortcuts and the classifier are stock torch ops, or, with pointwise="int8", all of them products in 8-bit integers
+(activations with a scale per pixel, weights with one per output channel).  With layout="NCHW" the layers of the two high-resolution
 stages (56x56 and 28x28) run as one kernel each, BatchNorms and shortcut add included (a shortcut that goes through a ReLU first gets
 it in a pass of its own there, and inside the last kernel elsewhere).  Weights are random (seeded): there is no checkpoint to load here.
 """
@@ -100,8 +101,11 @@ class _WinogradLayer(torch.nn.Module):
 
 
 class ResNet18Var(torch.nn.Module):
-    def __init__(self, num_classes=1000, stage5_pool=True, seed=0, math="tf32", fused=True, layout="NCHW"):
+    def __init__(self, num_classes=1000, stage5_pool=True, seed=0, math="tf32", fused=True, layout="NCHW", pointwise=None):
         super().__init__()
+        if pointwise not in (None, "int8"):
+            raise ValueError("pointwise must be None or \"int8\", got %r" % (pointwise,))
+        self.pointwise = pointwise      # the 1x1 shortcuts and the classifier
         gen = torch.Generator().manual_seed(seed)
         self.math = math
         # physical layout of the activations: "NCHW" (torch's default) lets the high-resolution layers run as one
@@ -148,6 +152,21 @@ class ResNet18Var(torch.nn.Module):
         t = conv(blk["w2b"], blk["bn2b"](t))
         return main + blk["bn2c"](t)
 
+    def _codes_of(self, owner, name, weights):
+        """quantize_int8 of the weights that the call gives, kept on `owner` until they are on another device"""
+        kept = getattr(owner, name, None)
+        if kept is None or kept[0].device != self.fc_w.device:
+            kept = wg2x2.quantize_int8(weights().detach().flatten(1).contiguous())
+            setattr(owner, name, kept)
+        return kept
+
+    def _shortcut_int8(self, blk, x, relu):
+        """bn1(conv1x1([relu]x)) in 8 bits, without bn1's shift where the block's last kernel adds it"""
+        w, w_scale = self._codes_of(blk, "_short_codes", lambda: blk.short * blk["bn1"].scale.view(-1, 1, 1, 1))
+        q, scale = wg2x2.quantize_int8(_WinogradLayer._to_kernel(x, self.layout), relu=relu, layout=self.layout)
+        y = wg2x2.linear_int8(q, scale, w, w_scale, bias=None if self.fused else blk["bn1"].shift, layout=self.layout)
+        return _WinogradLayer._from_kernel(y, self.layout)
+
     def forward(self, image, reference=False):
         """image: (B,3,H,W) float32, already normalised.  reference=True computes the Winograd layers with
         float64 einsums instead of this repository's kernels."""
@@ -183,12 +202,17 @@ class ResNet18Var(torch.nn.Module):
             l, l_relu = wg2x2.maxpool3x3s2_same(l, with_relu=True, relu_scale=pre.scale, relu_shift=pre.shift)
         else:
             l = _same_pool(l)
+        int8 = self.pointwise == "int8" and not reference and image.is_cuda
         for s, (blk_a, blk_b) in enumerate(self.blocks):
             if l_relu is not None:
                 main = l_relu
+            elif int8:
+                main = blk_a["pre"](l) if s == 0 else l         # (its ReLU in the quantiser)
             else:
                 main = torch.relu(blk_a["pre"](l)) if s == 0 else torch.relu(l)
-            if reference or not self.fused:
+            if int8:
+                main = self._shortcut_int8(blk_a, main, l_relu is None)
+            elif reference or not self.fused:
                 main = blk_a["bn1"](F.conv2d(main, blk_a.short))
             else:   # the BatchNorm after the 1x1 shortcut folds into its weights (once) and bias
                 if getattr(blk_a, "_short_folded", None) is None or blk_a._short_folded.device != blk_a.short.device:
@@ -209,6 +233,9 @@ class ResNet18Var(torch.nn.Module):
             l = wg2x2.relu_mean(l)
         else:
             l = torch.relu(l).mean(dim=(2, 3))
+        if int8:
+            q, scale = wg2x2.quantize_int8(l.contiguous())
+            return wg2x2.linear_int8(q, scale, *self._codes_of(self, "_fc_codes", lambda: self.fc_w), bias=self.fc_b)
         return F.linear(l, self.fc_w, self.fc_b)
 
     def winograd_layers(self):

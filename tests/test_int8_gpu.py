@@ -457,3 +457,49 @@ def test_largest_offsets():
     y = wg2x2.linear_int8(q, s, w, ws, dtype=torch.bfloat16)
     want, p = _linear_oracle(q[at], s[at], w, ws, None, False)
     _check_linear(y[at], want, p, torch.bfloat16)
+
+
+@pytest.mark.parametrize("layout,fused,stage5_pool", [("NCHW", True, True), ("NHWC", True, True), ("NCHW", False, False)])
+def test_network_with_pointwise_products_in_8_bits(layout, fused, stage5_pool, monkeypatch):
+    """ResNet18Var(pointwise="int8"): four shortcuts and the classifier, each what its operands say"""
+    import resnet18_var
+    net = resnet18_var.ResNet18Var(num_classes=100, layout=layout, fused=fused, stage5_pool=stage5_pool, pointwise="int8").cuda()
+    image = torch.randn((3, 3, 96, 96), generator=_gen("net"), device="cuda")
+    net(image)                                       # (the weights' codes are made once)
+    calls = []
+
+    def recorded(name):
+        f = getattr(wg2x2, name)
+
+        def g(*a, **k):
+            r = f(*a, **k)
+            calls.append((name, a, k, r if name == "quantize_int8" else r.clone()))      # (a block's last kernel writes over its shortcut)
+            return r
+        monkeypatch.setattr(wg2x2, name, g)
+    recorded("quantize_int8")
+    recorded("linear_int8")
+    logits = net(image)
+    assert logits.shape == (3, 100) and bool(logits.isfinite().all())
+    assert [c[0] for c in calls] == ["quantize_int8", "linear_int8"] * 5 and torch.equal(logits, calls[-1][3])
+    for i, (name, a, k, r) in enumerate(calls):
+        nchw = k.get("layout") == "NCHW"
+        if name == "quantize_int8":
+            x = a[0].permute(0, 2, 3, 1) if nchw else a[0]
+            rows = x.reshape(-1, x.shape[-1]).double()
+            q0, s0 = _codes(torch.relu(rows) if k.get("relu") else rows)
+            assert torch.equal(r[0].reshape(q0.shape), q0) and torch.equal(r[1].flatten(), s0.float())
+        else:
+            assert a[0] is calls[i - 1][3][0] and a[1] is calls[i - 1][3][1]
+            want, p = _linear_oracle(a[0].reshape(-1, a[0].shape[-1]), a[1].flatten(), a[2], a[3], k.get("bias"), False)
+            y = r.permute(0, 2, 3, 1) if nchw else r
+            _check_linear(y.reshape(want.shape), want, p, torch.float32)
+    blk = net.blocks[1][0]
+    q0, s0 = _codes((blk.short * blk["bn1"].scale.view(-1, 1, 1, 1)).flatten(1).double())
+    assert torch.equal(blk._short_codes[0], q0) and torch.equal(blk._short_codes[1], s0.float())
+    assert (calls[1][2]["bias"] is None) == fused
+
+
+def test_pointwise_is_refused_by_name():
+    import resnet18_var
+    with pytest.raises(ValueError):
+        resnet18_var.ResNet18Var(pointwise="int4")
