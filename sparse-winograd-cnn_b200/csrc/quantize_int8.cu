@@ -203,25 +203,33 @@ __device__ __forceinline__ void load_weights(const RowsParams &p, int c0, float 
     }
 }
 
-// The whole number nearest to 127 u / a where u inv, which is within 7.6e-6 of that, is close to half way between two: k + 1/2.  127 u and
-// (k + 1/2) a are compared as sums of two 32-bit numbers each: the high parts lie within a factor of two of each other and the low
-// ones have 8 bits, so every difference is exact.  Both sides are first scaled to where nothing overflows or is denormal.
-__device__ __noinline__ unsigned near_tie(float u, float inv, float a)
+// The code of u beyond doubt: the half way point next to u inv (which is within 7.6e-6 of 127 u / a) is compared with 127 u / a, or rather
+// 127 u with that many a, as sums of two 32-bit numbers each.  Where they are close the high parts lie within a factor of two of each
+// other and the low ones have 8 bits, so that every difference is exact.  `scale` moves both to where nothing overflows or is denormal.
+__device__ __forceinline__ unsigned sure_code(float u, float inv, float a, float scale)
 {
-    const float k = floorf(__fmul_rn(u, inv)), half = k + 0.5f, s = a >= 2.f ? 0x1p-64f : 0x1p64f;
-    u *= s;
-    a *= s;
-    const float p = __fmul_rn(127.f, u), q = __fmul_rn(half, a);
-    const float d = __fadd_rn(__fsub_rn(p, q), __fsub_rn(fmaf(127.f, u, -p), fmaf(half, a, -q)));
-    const int i = (int)k;
-    return (unsigned)(d > 0.f || (d == 0.f && (i & 1)) ? i + 1 : i);
+    const float r = __fsub_rn(fmaf(u, inv, kRound), kRound), e = fmaf(u, inv, -r), half = r + (e >= 0.f ? 0.5f : -0.5f);
+    const float v = u * scale, p = __fmul_rn(127.f, v), q = __fmul_rn(half, a);
+    const float d = __fadd_rn(__fsub_rn(p, q), __fsub_rn(fmaf(127.f, v, -p), fmaf(half, a, -q)));
+    const unsigned below = __float_as_uint((half - 0.5f) + kRound);
+    return below + (d > 0.f || (d == 0.f && (below & 1u)) ? 1u : 0u);
+}
+__device__ __noinline__ unsigned sure_word(float u0, float u1, float u2, float u3, float inv, float a)
+{
+    const float s = a >= 2.f ? 0x1p-64f : 0x1p64f, b = a * s;
+    return __byte_perm(__byte_perm(sure_code(u0, inv, b, s), sure_code(u1, inv, b, s), 0x0040),
+                       __byte_perm(sure_code(u2, inv, b, s), sure_code(u3, inv, b, s), 0x0040), 0x5410);
 }
 
 // Codes of N values, four a word.  inv = 127 / a rounded, so |u inv - 127 u / a| <= 127 * 2^-24 = 7.6e-6.  m holds the whole number
 // nearest to u inv, which the fused multiply-add rounds once; d, its distance, is exact to 3e-8.  Wherever |d| <= 0.49999 that number is
-// also the one nearest to 127 u / a; elsewhere near_tie says (u = a / 2 is common in 16-bit types, and there are rows with a tie in every
-// dozen values).  a below kTinyRow or not finite: inv = 0, and the caller clears the codes.
-template <int N>
+// also the one nearest to 127 u / a; elsewhere sure_word says.  a below kTinyRow or not finite: inv = 0, and the caller clears the codes.
+//
+// Values of 16-bit types (COARSE) are half way between two codes in nearly every row (u = a / 2; every second value where a's mantissa is a
+// multiple of 127), but never close to it without being there: for u, a of at most 11 bits 254 u / ((2 k + 1) a) is a quotient of whole
+// numbers below 2^19, so it is 1 or differs from it by 2^-19.  u inv, rounded twice, is within 2^-23 of 127 u / a, two units of its last
+// place (four below 1/2): rounded to a multiple of eight of them it is k + 1/2 where that is the case, and on its own side of it where not.
+template <int N, bool COARSE>
 __device__ __forceinline__ float fast_codes(const float (&u)[N], float inv, unsigned (&w)[N / 4], float off = 0.f)      // -> the largest |d|
 {
 #pragma unroll
@@ -229,8 +237,14 @@ __device__ __forceinline__ float fast_codes(const float (&u)[N], float inv, unsi
         unsigned r[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float x = u[4 * g + j], m = fmaf(x, inv, kRound);
-            off = fmaxf(off, fabsf(fmaf(x, inv, -__fsub_rn(m, kRound))));
+            const float x = u[4 * g + j];
+            float m;
+            if (COARSE) {
+                m = __fadd_rn(__uint_as_float((__float_as_uint(__fmul_rn(x, inv)) + 4u) & ~7u), kRound);
+            } else {
+                m = fmaf(x, inv, kRound);
+                off = fmaxf(off, fabsf(fmaf(x, inv, -__fsub_rn(m, kRound))));
+            }
             r[j] = __float_as_uint(m);
         }
         w[g] = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
@@ -241,16 +255,12 @@ template <int N>
 __device__ __forceinline__ void mend_codes(const float (&u)[N], float inv, float a, unsigned (&w)[N / 4])
 {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const float x = u[j], m = fmaf(x, inv, kRound);
-        if (fabsf(fmaf(x, inv, -__fsub_rn(m, kRound))) > kNearTie)
-            w[j / 4] = __byte_perm(w[j / 4], near_tie(x, inv, a), (j & 3) == 0 ? 0x3214 : (j & 3) == 1 ? 0x3240 : (j & 3) == 2 ? 0x3410 : 0x4210);
-    }
+    for (int g = 0; g < N / 4; ++g) w[g] = sure_word(u[4 * g], u[4 * g + 1], u[4 * g + 2], u[4 * g + 3], inv, a);
 }
-template <int N>
+template <int N, bool COARSE>
 __device__ __forceinline__ void code_words(const float (&u)[N], float inv, float a, unsigned (&w)[N / 4])
 {
-    if (fast_codes<N>(u, inv, w) > kNearTie) mend_codes<N>(u, inv, a, w);
+    if (fast_codes<N, COARSE>(u, inv, w) > kNearTie) mend_codes<N>(u, inv, a, w);
 }
 
 struct RowCodes {
@@ -497,7 +507,7 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256, !BLOCK &&
         unsigned w[V][WORDS];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            code_words<N>(u[v], k.inv, k.a, w[v]);
+            code_words<N, MODE == kQuantize && N == 8>(u[v], k.inv, k.a, w[v]);
 #pragma unroll
             for (int g = 0; g < WORDS; ++g) w[v][g] &= k.live;
         }
@@ -563,7 +573,7 @@ __global__ void __launch_bounds__(512) rows_any_kernel(const RowsParams p)
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
         const float u[4] = {value(c), 0.f, 0.f, 0.f};
         unsigned w[1];
-        code_words<4>(u, k.inv, k.a, w);
+        code_words<4, MODE == kQuantize && sizeof(T) == 2>(u, k.inv, k.a, w);
         q[c] = (signed char)(w[0] & k.live);
     }
 }
@@ -708,7 +718,7 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
         unsigned w[KEEP][1];
         float off = 0.f;
 #pragma unroll
-        for (int g = 0; g < KEEP; ++g) off = fast_codes<4>(u[g], k.inv, w[g], off);
+        for (int g = 0; g < KEEP; ++g) off = fast_codes<4, MODE == kQuantize && sizeof(T) == 2>(u[g], k.inv, w[g], off);
         if (off > kNearTie) {
 #pragma unroll
             for (int g = 0; g < KEEP; ++g) mend_codes<4>(u[g], k.inv, k.a, w[g]);
@@ -751,7 +761,7 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
                 v[j] = c < C ? value(to_f((MODE == kNormRes ? h : x)[c * HW]), c) : 0.f;
             }
             unsigned codes[1];
-            code_words<4>(v, k.inv, k.a, codes);
+            code_words<4, MODE == kQuantize && sizeof(T) == 2>(v, k.inv, k.a, codes);
             const unsigned w = codes[0] & k.live;
             signed char *dst = p.Q + row * p.ldq + 4 * q;
 #pragma unroll
@@ -799,12 +809,11 @@ static int rows_int8(RowsParams p, cudaStream_t st)
     const bool odd = ox || p.C % N || p.ldq % N || (reinterpret_cast<uintptr_t>(p.Q) & (N - 1));
     const long long nv = odd ? cdivll((long long)p.C + N - 1, N) : p.C / N;
     if (!same || nv > 4096) return launch(rows_any_kernel<T, MODE>, dim3((unsigned)p.rows), 512, 0, st, p);
-    // A few rows: as many threads a row as it has loads.  Many: a row in a warp or a part of one up to 128 loads, else four or eight loads a
-    // thread.
-    const bool few = p.rows < 2 * kNumSMs;
-    if (few && nv > 32 && nv <= 1024) return launch_rows<T, MODE, 1, true, 0>(odd, (int)(cdivll(nv, 32) * 32), p, st);
+    // Rows that fit the GPU at once with a thread for every load are taken so; else a row in a warp or a part of one up to 128 loads, and four
+    // or eight loads a thread.
+    const bool little = p.rows * nv <= 2048LL * kNumSMs;
+    if (little && nv > 32 && nv <= 1024) return launch_rows<T, MODE, 1, true, 0>(odd, (int)(cdivll(nv, 32) * 32), p, st);
     if (nv <= 128) {
-        const bool little = p.rows * nv < 8 * 256 * kNumSMs;       // less than a round of blocks of four loads a thread
         const int V = little ? 1 : nv >= 8 ? 4 : nv >= 4 ? 2 : 1;
         for (p.group = 2; p.group < 32 && p.group * V < nv;) p.group *= 2;
         if (p.group * V >= nv) {
