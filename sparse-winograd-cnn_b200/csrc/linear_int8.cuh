@@ -751,7 +751,7 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     const LiClusters clusters = li_clusters();
     li_choose(p, clusters);
     const int pairs = clusters.n[1];
-    if ((long long)p.lane_tiles * p.col_tiles > 0x3fffffffLL) return WG2X2_ERR_UNSUPPORTED;
+    if ((long long)p.lane_tiles * p.col_tiles > 0x3fffffffLL || p.col_tiles > 0x3ffffff) return WG2X2_ERR_UNSUPPORTED;
     const int b_rows = p.pair ? p.N / 2 : p.N, stage = (kBlockM + b_rows) * kLiChunk, other = 1024 + kLiCtrl + (p.splits > 1 ? p.N * kBlockM * 4 : 0);
     p.stages = std::min({kLiMaxStages, (kLiSmem - other) / stage, std::max(2, p.splits > 1 ? cdiv(p.chunks, p.splits) : kLiMaxStages)});
     p.spin_limit = wait_limit();
@@ -760,7 +760,9 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     const void *A = nchw ? Q : W, *Bop = nchw ? W : Q;
     const long long lda = nchw ? ldq : ldw, ldb = nchw ? ldw : ldq;
     if (!make_map_codes(&mapA, A, C, p.lanes, lda, kBlockM) || !make_map_codes(&mapB, Bop, C, p.cols, ldb, b_rows)) return WG2X2_ERR_LAUNCH;
-    const size_t smem = (size_t)other + (size_t)p.stages * stage;
+    // More than half of an SM's shared memory, whatever the tile: two CTAs that share an SM would wait for each other's tensor memory, and
+    // with CTAs of their clusters on other SMs, that wait in turn, without an end
+    const size_t smem = std::max((size_t)other + (size_t)p.stages * stage, (size_t)120 * 1024);
     if (type == WG2X2_F32) return nchw ? li_launch<true, float>(mapA, mapB, p, pairs, smem, st) : li_launch<false, float>(mapA, mapB, p, pairs, smem, st);
     if (type == WG2X2_F16) return nchw ? li_launch<true, __half>(mapA, mapB, p, pairs, smem, st) : li_launch<false, __half>(mapA, mapB, p, pairs, smem, st);
     return nchw ? li_launch<true, __nv_bfloat16>(mapA, mapB, p, pairs, smem, st) : li_launch<false, __nv_bfloat16>(mapA, mapB, p, pairs, smem, st);

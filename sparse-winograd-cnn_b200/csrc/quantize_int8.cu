@@ -865,6 +865,7 @@ static int codes_int8(int mode, int type, RowsParams &p, long long B, int HW, in
     p.C = C;
     p.HW = HW;
     if (!p.rows) return WG2X2_OK;
+    if (C > 1 << 30) return WG2X2_ERR_UNSUPPORTED;          // (a channel's index and a step beyond it fit 32 bits)
     const int e = type == WG2X2_F32 ? 4 : 2;
     const bool nchw = layout == WG2X2_NCHW;
     if (!p.X || !p.Q || !p.scale || (mode != kQuantize && !p.Wt) || (mode == kNormRes && (!p.R || !p.H))) return WG2X2_ERR_BAD_ARG;

@@ -425,6 +425,71 @@ def test_streams_threads_and_graphs():
     assert not bad
 
 
+def test_shared_tiles_on_several_streams():
+    """Products whose tiles are shared by clusters, many of them at once: no two wait for each other"""
+    g = _gen("several")
+    shapes = [(8, 1024, 256), (16, 4096, 128), (40, 2048, 512), (100, 8192, 1024), (9, 640, 64)]
+    sets = []
+    for rows, C, K in shapes:
+        q, w = _rand_codes(g, rows, C), _rand_codes(g, K, C)
+        sets.append((q, torch.rand(rows, generator=g, device="cuda"), w, torch.rand(K, generator=g, device="cuda")))
+    want = [wg2x2.linear_int8(*a) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    got = []
+    for i in range(60):
+        with torch.cuda.stream(streams[i % 6]):
+            k = (i * 7 + i // 6) % len(sets)
+            got.append((k, wg2x2.linear_int8(*sets[k])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[k]) for k, y in got) and wg2x2.last_device_status()[0] == 0
+
+
+_FIRST_CALL = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+import wg2x2
+x, res = torch.randn((300, 1000), device="cuda"), torch.randn((300, 1000), device="cuda")
+w, one = torch.randn((500, 1000), device="cuda"), torch.ones(1000, device="cuda")
+im = torch.randn((2, 64, 9, 9), device="cuda")
+torch.cuda.synchronize()
+def f():
+    q, s, h = wg2x2.rms_norm_int8(x, one, residual=res)
+    t = wg2x2.quantize_int8(w)
+    return wg2x2.linear_int8(q, s, *t), wg2x2.linear_int8(q[:8], s[:8], *t), wg2x2.linear_int8(q[:2], s[:2], *t), h, wg2x2.quantize_int8(im, layout="NCHW")[0]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = f()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(y, f()))
+print("same")
+"""
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sparse-winograd-cnn_b200")
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL, pkg], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_other_current_stream_and_reused_memory():
+    """A result's memory goes back to its stream's pool while kernels that read it are queued there: in order, so nothing is disturbed"""
+    g = _gen("reuse")
+    w = wg2x2.quantize_int8(torch.randn((256, 512), generator=g, device="cuda"))
+    x = torch.randn((64, 512), generator=g, device="cuda")
+    want = wg2x2.linear_int8(*wg2x2.quantize_int8(x), *w)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+        ys = [wg2x2.linear_int8(*wg2x2.quantize_int8(x), *w) for _ in range(50)]
+        torch.cuda.current_stream().synchronize()
+    assert all(torch.equal(y, want) for y in ys)
+
+
 @pytest.mark.parametrize("rows,C,K", [(9, 4096, 256), (3000, 256, 1024), (6000, 1024, 4096)])
 def test_time_out_of_the_product(rows, C, K):
     """A load that never comes: the wait for it gives up, the status says so, and the next call is right"""
