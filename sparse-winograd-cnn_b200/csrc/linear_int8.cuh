@@ -12,13 +12,13 @@
 // the shares (whole numbers, so the order does not matter) meet through distributed shared memory, every CTA finishing N / S columns.
 #pragma once
 
-constexpr int kLiEpiWarps = 16;               // four for each quarter of the lanes: a product with few channels is all epilogue
+constexpr int kLiEpiWarps = 16;               // two sets of eight, one for each accumulator: a product with few channels is all epilogue
 constexpr int kLiThreads = 32 * (2 + kLiEpiWarps);       // producer, MMA issuer, epilogue
 constexpr int kLiChunk = 128;                 // bytes of the contraction a stage
 constexpr int kLiMaxStages = 12;
 constexpr int kLiSmem = 232448;               // all that a CTA can have
-constexpr int kLiAhead = 4;
-constexpr int kLiCorner = 64;                 // columns of a tile that an epilogue warp finishes, at most
+constexpr int kLiAhead = 2;
+constexpr int kLiCorner = 128;                // columns of a tile that an epilogue warp finishes, at most
 constexpr int kLiCtrl = 512 + kLiEpiWarps * 2 * kLiCorner * 4;     // barriers; the scales and biases of those columns, for each epilogue warp
 constexpr int kLiMaxC = 131071;
 
@@ -200,25 +200,32 @@ __device__ __forceinline__ void li_store(const LiParams &p, const LiLane<NCHW, T
     }
 }
 
-// What an epilogue warp does with the tiles first, first + step, ... of `lanes_tile` lanes; the CTA's begin at lane0 of them.  accf, acce:
-// barriers of the first accumulator, those of the second 8 bytes further; `release` hands an accumulator back.  False: gave up waiting.
+// What epilogue warp 0 .. 15 (the CTA's warps from 2 on) does with its tiles of first, first + step, ..., of `lanes_tile` lanes; the CTA's
+// begin at lane0 of them.  Every second tile is in the second accumulator, and warps 8 .. 15's, so that one set waits for its tile, or for
+// tensor memory, while the other computes and stores.  accf, acce: barriers of the first accumulator, those of the second 8 bytes further;
+// `release` hands an accumulator back.  False: gave up waiting.
+// Bound, where the contraction is short, by the result's way to memory: 200704 x 64 -> 128, NCHW in 32 bits, 25.5 us, 15.4 without its stores
+// (103 MB, which a plain fill writes in 18); two stores of half as many instructions each, or eight warps in all, measured the same.
 template <bool NCHW, typename T, typename Release>
-__device__ __forceinline__ bool li_epilogue(const LiParams &prm, int first, int step, int lanes_tile, int lane0, int part, int q, int lane, float *corner,
+__device__ __forceinline__ bool li_epilogue(const LiParams &prm, int first, int step, int lanes_tile, int lane0, int warp, int lane, float *corner,
                                             uint32_t tmem, uint32_t accf, uint32_t acce, volatile int *abort_flag, Release release)
 {
-    const int units = prm.lane_tiles * prm.col_tiles, width = max(32, prm.N / 4);
+    const int set = warp >> 3, part = (warp >> 2) & 1, q = (warp + 2) & 3;      // (a warp reads the lanes 32 (its number in the CTA & 3) on)
+    const int units = prm.lane_tiles * prm.col_tiles, width = max(32, prm.N / 2);
     const int c_tile = part * width, ncols = min(width, prm.N - c_tile);         // the warp's columns of a tile (none: ncols <= 0)
     // A tile with a short contraction takes less time than a load from memory: the lanes' scales are asked for kLiAhead tiles ahead
     LiScale ahead[kLiAhead];
-    int lt, ct, col_now = -1, buf = 0;
+    int lt, ct, col_now = -1;
     uint32_t use = 0;
+    auto at = [&](int u, int k) { return (int)min((long long)units - 1, u + 2LL * k * step); };
+    first += set * step;
 #pragma unroll
     for (int k = 0; k < kLiAhead; ++k) {
-        li_decode(prm, (int)min((long long)units - 1, first + (long long)k * step), lt, ct);
+        li_decode(prm, at(first, k), lt, ct);
         ahead[k] = li_lane_scale<NCHW>(prm, lt * lanes_tile + lane0 + q * 32 + lane);
     }
     LiColumns<NCHW> columns;
-    for (int u = first; u < units; u += step) {
+    for (int u = first; u < units; u += 2 * step) {
         li_decode(prm, u, lt, ct);
         const LiLane<NCHW, T> me(prm, lt * lanes_tile + lane0 + q * 32 + lane, ahead[0]);
         const int col0 = ct * prm.N + c_tile;
@@ -229,16 +236,15 @@ __device__ __forceinline__ bool li_epilogue(const LiParams &prm, int first, int 
             columns.put(corner, lane);
             col_now = col0;
         }
-        li_decode(prm, (int)min((long long)units - 1, u + (long long)kLiAhead * step), lt, ct);
+        li_decode(prm, at(u, kLiAhead), lt, ct);
         ahead[kLiAhead - 1] = li_lane_scale<NCHW>(prm, lt * lanes_tile + lane0 + q * 32 + lane);
-        if (!mbar_wait_warp(accf + 8u * buf, use & 1u, abort_flag, 0x1F00u | buf, prm.spin_limit)) return false;
+        if (!mbar_wait_warp(accf + 8u * set, use & 1u, abort_flag, 0x1F00u | set, prm.spin_limit)) return false;
         tc_fence_after();
-        li_store<NCHW, T>(prm, me, tmem + (uint32_t)(buf * 256 + c_tile), corner, col0, ncols);
+        li_store<NCHW, T>(prm, me, tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(set * 256 + c_tile), corner, col0, ncols);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) release(acce + 8u * buf);
-        buf ^= 1;
-        if (buf == 0) ++use;
+        if (lane == 0) release(acce + 8u * set);
+        ++use;
     }
     return true;
 }
@@ -280,7 +286,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
     const int early = prm.drop_load >= 0 ? 0 : min(prm.stages, kend - kbeg);
     if (threadIdx.x == 0) {
         for (int s = 0; s < prm.stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), kLiEpiWarps); }
+        for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), kLiEpiWarps / 2); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         int lt, ct;
@@ -358,7 +364,7 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
         float *corner = reinterpret_cast<float *>(ctrl_gen + 512) + (warp - 2) * 2 * kLiCorner;
         const uint32_t quarter = (uint32_t)(q * 32) << 16;
         if (!SPLIT) {
-            ok = li_epilogue<NCHW, T>(prm, first, step, kBlockM, 0, part, q, lane, corner, tmem_base + quarter, accf_bar(0), acce_bar(0), abort_flag,
+            ok = li_epilogue<NCHW, T>(prm, first, step, kBlockM, 0, warp - 2, lane, corner, tmem_base, accf_bar(0), acce_bar(0), abort_flag,
                                       [](uint32_t bar) { mbar_arrive(bar); });
         } else {
             // this CTA's share of the sums to the CTAs that finish them: [share][column][lane]
@@ -416,7 +422,9 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
 
 // The same on pairs of SMs (tcgen05 cta_group::2) for tiles of 256 lanes x N columns: each CTA of a cluster of two has 128 of the lanes and
 // brings half of B, which the tensor cores exchange, so that 256 columns take 32 KB of operands a chunk and SM instead of 48: at one CTA a
-// tile it is the operands' way from L2 that the products wait for.  Barriers as in conv_tc_gemm2.cuh: `full` in the leader counts both
+// tile it is the operands' way from L2 that the products wait for.  8192 x 4096 x 4096: 89.8 us = 3060 T/s at full clock, tensor pipe busy
+// 78 % of the time, operands at 47 bytes a clock and SM (one CTA a tile: 95 us; back to back for seconds, under the power limit: 103 and
+// 112).  Barriers as in conv_tc_gemm2.cuh: `full` in the leader counts both
 // CTAs' bytes, `empty` and `accf` are committed to both, `acce` in the leader counts the epilogue warps of both.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t cluster_bar, int c0, int c1)
 {
@@ -452,7 +460,7 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_c
     const uint32_t rank = cluster_ctarank();
     if (threadIdx.x == 0) {
         for (int s = 0; s < prm.stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), 2 * kLiEpiWarps); }
+        for (int b = 0; b < 2; ++b) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), kLiEpiWarps); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -522,10 +530,8 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_c
             if (!ok) let_them_land();
         }
     } else {
-        const int q = warp & 3, part = (warp - 2) >> 2;
         float *corner = reinterpret_cast<float *>(ctrl_gen + 512) + (warp - 2) * 2 * kLiCorner;
-        li_epilogue<NCHW, T>(prm, first, step, 256, (int)rank * kBlockM, part, q, lane, corner, tmem_base + ((uint32_t)(q * 32) << 16), accf_bar(0), acce_bar(0),
-                             abort_flag, [](uint32_t bar) { mbar_arrive_cluster(mapa_rank0(bar)); });
+        li_epilogue<NCHW, T>(prm, first, step, 256, (int)rank * kBlockM, warp - 2, lane, corner, tmem_base, accf_bar(0), acce_bar(0), abort_flag, [](uint32_t bar) { mbar_arrive_cluster(mapa_rank0(bar)); });
     }
     // Neither CTA may leave, or free its tensor memory, while the other can still read its shared memory through an MMA or signal one of its
     // barriers
@@ -540,7 +546,9 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_c
 
 // A few rows of codes: nothing but the weights' bytes counts, and the set-up of the kernels above (tensor memory, barriers, a cluster's
 // exchange) would take longer than those.  `group` lanes have a row of weights, 16 bytes a load and eight loads on their way, and multiply
-// four codes an instruction.
+// four codes an instruction.  1, 2, 3, 4 rows against the kernels above, us in a graph: 4096 x 4096 (16.8 MB, 2.6 us of memory) 3.2, 4.4,
+// 6.0, 6.5 / 7.4; 512 x 1000 2.1, 2.6, 3.4, 3.4 / 4.6; 8192 x 8192 (10.2 us) 14.5, 15.1, 16.5, 16.5 / 15.8.  Eight rows: 10.3 / 7.4, 5.2 /
+// 4.7, 37.6 / 16.1 (the codes' loads, one for every two rows of weights).
 constexpr int kLiFewRows = 4;
 struct LiFewParams {
     const signed char *Q, *W;
