@@ -20,7 +20,6 @@
 
 #include <algorithm>
 
-
 #include "wg_common.cuh"
 
 namespace wg {
@@ -294,7 +293,8 @@ __device__ __forceinline__ float norm_scale(const RowCodes &k, float ss, int C, 
     return __fdiv_rn(scale, __fsqrt_rn(mean + eps));
 }
 
-// The largest magnitude and the sum over `width` lanes (8, 16 or 32)
+// The largest magnitude and the sum over `width` lanes (2 to 32).  By shuffles: the warp's own reduction (__reduce_max_sync), behind the ends
+// of a row that some lanes handle apart, left out what those lanes had.
 template <bool SUM>
 __device__ __forceinline__ void reduce_lanes(float &a, float &ss, int width)
 {
@@ -813,10 +813,10 @@ static int rows_int8(RowsParams p, cudaStream_t st)
     const bool odd = ox || p.C % N || p.ldq % N || (reinterpret_cast<uintptr_t>(p.Q) & (N - 1));
     const long long nv = odd ? cdivll((long long)p.C + N - 1, N) : p.C / N;
     if (!same || nv > 4096) return launch(rows_any_kernel<T, MODE>, dim3((unsigned)p.rows), 512, 0, st, p);
-    // Rows that fit the GPU at once with a thread for every load are taken so (norm of 300 x 1024 bf16: 2.6 us, the other way 6.6; of
-    // 4000 x 1024 the other way: 9.7); else a row in a warp or a part of one up to 128 loads, and four
+    // Rows that fit the GPU at once with a thread for every load (1024 threads an SM) are taken so: norm with a shortcut, us in a graph,
+    // 300 x 1024 bf16 2.4, the other way 4.4; beyond the bound 2000 x 1283 bf16 10.6 and 8.9, 600 x 1283 float 6.9 and 4.5.  Else a row in a warp or a part of one up to 128 loads, and four
     // or eight loads a thread.
-    const bool little = p.rows * nv <= 2048LL * kNumSMs;
+    const bool little = p.rows * nv <= 1024LL * kNumSMs;
     if (little && nv > 32 && nv <= 1024) return launch_rows<T, MODE, 1, true, 0>(odd, (int)(cdivll(nv, 32) * 32), p, st);
     if (nv <= 128) {
         const int V = little ? 1 : nv >= 8 ? 4 : nv >= 4 ? 2 : 1;
