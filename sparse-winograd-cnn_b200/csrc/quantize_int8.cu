@@ -534,25 +534,26 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256, !BLOCK &&
     }
 }
 
-// Rows of any length and alignment, value by value; read a second time for the codes (from L2): what rows_kernel does not hold.
-template <typename T, int MODE>
+// Rows of any length and alignment, value by value; read a second time for the codes (from L2): what rows_kernel does not hold, and, with
+// NCHW, images of more channels than nchw_kernel's shared memory takes codes of (some 6000).
+template <typename T, int MODE, bool NCHW>
 __global__ void __launch_bounds__(512) rows_any_kernel(const RowsParams p)
 {
     __shared__ float2 part[2 * 32];
     wait_for_previous_kernel(kNumSMs);
-    const long long row = blockIdx.x;
-    const T *x = static_cast<const T *>(p.X) + row * p.ldx;
-    const T *res = MODE == kNormRes ? static_cast<const T *>(p.R) + row * p.ldr : nullptr;
-    T *h = MODE == kNormRes ? static_cast<T *>(p.H) + row * p.ldh : nullptr;
+    const long long row = blockIdx.x, step = NCHW ? p.HW : 1, pixel = NCHW ? row / p.HW * p.C * p.HW + row % p.HW : 0;
+    const T *x = static_cast<const T *>(p.X) + (NCHW ? pixel : row * p.ldx);
+    const T *res = MODE == kNormRes ? static_cast<const T *>(p.R) + (NCHW ? pixel : row * p.ldr) : nullptr;
+    T *h = MODE == kNormRes ? static_cast<T *>(p.H) + (NCHW ? pixel : row * p.ldh) : nullptr;
     const T *again = MODE == kNormRes ? h : x;
     auto value = [&](int c) {
-        const float v = to_f(again[c]);
+        const float v = to_f(again[c * step]);
         return MODE != kQuantize ? __fmul_rn(v, weight_at(p, (const T *)nullptr, c)) : p.relu ? relu_nan(v) : v;
     };
     float amax = 0.f, ss = 0.f;
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
-        if (MODE == kNormRes) h[c] = from_f<T>(__fadd_rn(to_f(x[c]), to_f(res[c])));
-        const float v = to_f(again[c]);
+        if (MODE == kNormRes) h[c * step] = from_f<T>(__fadd_rn(to_f(x[c * step]), to_f(res[c * step])));
+        const float v = to_f(again[c * step]);
         ss = fmaf(v, v, ss);
         amax = mag_max(amax, value(c));
     }
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(512) rows_any_kernel(const RowsParams p)
             float none = 0.f;
             ss = 0.f;
             for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
-                const float f = to_f(again[c]) * kDown;
+                const float f = to_f(again[c * step]) * kDown;
                 ss = fmaf(f, f, ss);
             }
             reduce_block<true>(none, ss, part + 32);
@@ -590,7 +591,7 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
 {
     extern __shared__ unsigned turned_all[];        // [tile of the block][32][pitch], then the weights
     __shared__ float2 part[2][16][32];
-    constexpr bool SUM = MODE != kQuantize;
+    constexpr bool SUM = MODE != kQuantize, COARSE = MODE == kQuantize && sizeof(T) == 2;
     wait_for_previous_kernel(kNumSMs);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = p.group;
     const int tile = warp / share, wi = warp - tile * share, tiles = (blockDim.x >> 5) / share;
@@ -611,48 +612,72 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
     const int C = p.C, words = (C + 3) >> 2, pitch = words | 1;
     const long long HW = p.HW;
     const float low = p.relu ? 0.f : __uint_as_float(0xff800000u);
-    auto value = [&](float v, int c) { return MODE != kQuantize ? __fmul_rn(v, weight_at(p, (const T *)nullptr, c)) : at_least(v, low); };
     float *weights = reinterpret_cast<float *>(turned_all) + tiles * 32 * pitch;
-    if (NQ && SUM) {
+    auto stage_weights = [&] {          // (behind the pixels' loads where those are all at hand)
         for (int c = threadIdx.x; c < 4 * words; c += blockDim.x) weights[c] = c < C ? weight_at(p, (const T *)nullptr, c) : 0.f;
         __syncthreads();
-    }
+    };
+    if (SUM && !NQ) stage_weights();
 
-    constexpr int KEEP = NQ ? NQ : 1;
+    constexpr int KEEP = NQ ? NQ : 1, LOOP = 4;
     float u[KEEP][4];
     float amax = 0.f, ss = 0.f;
     if (NQ) {
-        // the thread's groups of four channels: wi, wi + share, ...; FULL: all of them exist, with all four
-        const long long step = 4 * share * HW, at0 = 4 * wi * HW;
-        auto load = [&](const T *t, float (&v)[4], int g) {
-            if (FULL) {
+        // The thread's groups of four channels: wi, wi + share, ...  FULL: all of them exist.  Else those from `whole` on are read like the
+        // last whole one, which costs nothing beside loads behind conditions, and replaced: by the up to three channels that are left, which
+        // are read apart, and by zeros.
+        const long long step = 4 * share * HW;
+        const int whole = C >> 2;
+        auto load = [&](const T *base, float (&v)[4], int g) {
+            const T *t = base + (FULL ? g * step + 4 * wi * HW : 4LL * min(wi + g * share, whole - 1) * HW);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = to_f(t[j * HW]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = 4 * (wi + g * share) + j < C ? to_f(t[j * HW]) : 0.f;
-            }
+            for (int j = 0; j < 4; ++j) v[j] = to_f(t[j * HW]);
         };
-        const T *t = x + at0;
+        auto load_rest = [&](const T *base, float (&v)[4]) {
 #pragma unroll
-        for (int g = 0; g < KEEP; ++g, t += step) load(t, u[g], g);
+            for (int j = 0; j < 4; ++j) v[j] = 4 * whole + j < C ? to_f(base[(4LL * whole + j) * HW]) : 0.f;
+        };
+        auto replace = [&](float (&v)[4], const float (&rest)[4], int g) {
+            const int q = wi + g * share;
+            if (FULL || q < whole) return;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = q == whole ? rest[j] : 0.f;
+        };
+        float rest[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < KEEP; ++g) load(x, u[g], g);
+        if (!FULL && (C & 3)) load_rest(x, rest);
+#pragma unroll
+        for (int g = 0; g < KEEP; ++g) replace(u[g], rest, g);
+        if (SUM) stage_weights();
         if (MODE == kNormRes) {
             constexpr int HALF = KEEP > 8 ? 8 : KEEP;
-            const T *t = res + at0;
-            T *o = h + at0;
 #pragma unroll
             for (int g0 = 0; g0 < KEEP; g0 += HALF) {
                 float r[HALF][4];
 #pragma unroll
-                for (int g = 0; g < HALF; ++g, t += step) load(t, r[g], g0 + g);
+                for (int g = 0; g < HALF; ++g) load(res, r[g], g0 + g);
+                if (!FULL && (C & 3)) load_rest(res, rest);
 #pragma unroll
-                for (int g = 0; g < HALF; ++g, o += step)
+                for (int g = 0; g < HALF; ++g) {
+                    replace(r[g], rest, g0 + g);
+                    const int left = have ? C - 4 * (wi + (g0 + g) * share) : 0;
+                    T *o = h + 4LL * (wi + (g0 + g) * share) * HW;
+                    T s[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const T s = from_f<T>(__fadd_rn(u[g0 + g][j], r[g][j]));
-                        if (have && (FULL || 4 * (wi + (g0 + g) * share) + j < C)) o[j * HW] = s;
-                        u[g0 + g][j] = to_f(s);
+                        s[j] = from_f<T>(__fadd_rn(u[g0 + g][j], r[g][j]));
+                        u[g0 + g][j] = to_f(s[j]);
                     }
+                    if (FULL ? have : left >= 4) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[j * HW] = s[j];
+                    } else if (!FULL && left > 0) {
+#pragma unroll
+                        for (int j = 0; j < 3; ++j)
+                            if (j < left) o[j * HW] = s[j];
+                    }
+                }
             }
         }
 #pragma unroll
@@ -674,16 +699,29 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
             for (int j = 0; j < 4; ++j) amax = mag_max(amax, u[g][j]);
         }
     } else {
-        for (int c = wi; c < C; c += share) {
-            const long long o = c * HW;
-            float v = to_f(x[o]);
-            if (MODE == kNormRes) {
-                const T s = from_f<T>(__fadd_rn(v, to_f(res[o])));
-                if (have) h[o] = s;
-                v = to_f(s);
-            }
-            ss = fmaf(v, v, ss);
-            amax = mag_max(amax, value(v, c));
+        for (int q0 = wi; q0 < words; q0 += LOOP * share) {
+            float v[LOOP][4], r[LOOP][4];
+#pragma unroll
+            for (int g = 0; g < LOOP; ++g)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = 4 * (q0 + g * share) + j;
+                    v[g][j] = c < C ? to_f(x[c * HW]) : 0.f;
+                    if (MODE == kNormRes) r[g][j] = c < C ? to_f(res[c * HW]) : 0.f;
+                }
+#pragma unroll
+            for (int g = 0; g < LOOP; ++g)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = 4 * (q0 + g * share) + j;
+                    if (MODE == kNormRes) {
+                        const T s = from_f<T>(__fadd_rn(v[g][j], r[g][j]));
+                        if (have && c < C) h[c * HW] = s;
+                        v[g][j] = to_f(s);
+                    }
+                    if (SUM) ss = fmaf(v[g][j], v[g][j], ss);
+                    amax = mag_max(amax, SUM ? (c < C ? __fmul_rn(v[g][j], weights[c]) : 0.f) : at_least(v[g][j], low));
+                }
         }
     }
     // a pixel's maximum and sum over the warps that share it; each of them adds in the same order
@@ -717,60 +755,74 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
     } else if (wi == 0 && have) {
         p.scale[row] = row_scale(k);
     }
+    unsigned *turned = turned_all + tile * 32 * pitch;
     if (NQ) {
-        unsigned *turned = turned_all + tile * 32 * pitch;
         unsigned w[KEEP][1];
         float off = 0.f;
 #pragma unroll
-        for (int g = 0; g < KEEP; ++g) off = fast_codes<4, MODE == kQuantize && sizeof(T) == 2>(u[g], k.inv, w[g], off);
+        for (int g = 0; g < KEEP; ++g) off = fast_codes<4, COARSE>(u[g], k.inv, w[g], off);
         if (off > kNearTie) {
 #pragma unroll
-            for (int g = 0; g < KEEP; ++g) mend_codes<4>(u[g], k.inv, k.a, w[g]);
+            for (int g = 0; g < KEEP; ++g) code_words<4, COARSE>(u[g], k.inv, k.a, w[g]);       // (each word with a look of its own)
         }
 #pragma unroll
         for (int g = 0; g < KEEP; ++g) {
             const int q = wi + g * share;
             if (FULL || q < words) turned[lane * pitch + q] = w[g][0] & k.live;
         }
+    } else {
+        const T *again = MODE == kNormRes ? h : x;          // (what this thread itself has read or stored)
+        for (int q0 = wi; q0 < words; q0 += LOOP * share) {
+            float v[LOOP][4];
+#pragma unroll
+            for (int g = 0; g < LOOP; ++g)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = 4 * (q0 + g * share) + j;
+                    v[g][j] = c < C ? to_f(again[c * HW]) : 0.f;
+                }
+#pragma unroll
+            for (int g = 0; g < LOOP; ++g) {
+                const int q = q0 + g * share;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[g][j] = SUM ? (4 * q + j < C ? __fmul_rn(v[g][j], weights[4 * q + j]) : 0.f) : at_least(v[g][j], low);
+                unsigned w[1];
+                code_words<4, COARSE>(v[g], k.inv, k.a, w);
+                if (q < words) turned[lane * pitch + q] = w[0] & k.live;
+            }
+        }
+    }
+    {
         if (share == 1) __syncwarp();
         else __syncthreads();
         const int n = row0 < p.rows ? (int)min(32LL, p.rows - row0) : 0;
         signed char *rows = p.Q + row0 * p.ldq;
         const unsigned align = (unsigned)reinterpret_cast<uintptr_t>(p.Q) | (unsigned)p.ldq;
-        // pieces of 16 bytes, else words, the last one of a row byte by byte; i / pieces = the high word of i * inv
-        const bool by16 = p.C % 16 == 0 && (align & 15u) == 0;
-        const int pieces = by16 ? words >> 2 : words;
+        // pieces of 16 bytes, and what is left of a row by the lane of its number; else words, the last one byte by byte.  i / pieces = the
+        // high word of i * inv
+        const bool by16 = (align & 15u) == 0;
+        const int pieces = by16 ? C >> 4 : words;
         for (int i = 32 * wi + lane; i < n * pieces; i += 32 * share) {
             const int r = pieces == 1 ? i : (int)__umulhi((unsigned)i, p.inv), q = i - r * pieces;
             const unsigned *src = turned + r * pitch + (by16 ? 4 * q : q);
             signed char *dst = rows + r * p.ldq + (by16 ? 16 * q : 4 * q);
             if (by16) {
                 *reinterpret_cast<uint4 *>(dst) = make_uint4(src[0], src[1], src[2], src[3]);
-            } else if ((align & 3u) == 0 && 4 * q + 4 <= p.C) {
+            } else if ((align & 3u) == 0 && 4 * q + 4 <= C) {
                 *reinterpret_cast<unsigned *>(dst) = *src;
             } else {
                 const unsigned w = *src;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (4 * q + j < p.C) dst[j] = (signed char)(w >> (8 * j));
+                    if (4 * q + j < C) dst[j] = (signed char)(w >> (8 * j));
             }
         }
-    } else {
-        // (h as any warp stored it: over_warps is a barrier)
-        for (int q = wi; have && 4 * q < C; q += share) {
-            float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = 4 * q + j;
-                v[j] = c < C ? value(to_f((MODE == kNormRes ? h : x)[c * HW]), c) : 0.f;
-            }
-            unsigned codes[1];
-            code_words<4, MODE == kQuantize && sizeof(T) == 2>(v, k.inv, k.a, codes);
-            const unsigned w = codes[0] & k.live;
-            signed char *dst = p.Q + row * p.ldq + 4 * q;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (4 * q + j < C) dst[j] = (signed char)(w >> (8 * j));
+        if (by16 && (C & 15) && wi == share - 1 && lane < n) {
+            const unsigned *src = turned + lane * pitch;
+            signed char *dst = rows + lane * p.ldq;
+            int q = pieces * 4;
+            for (; 4 * q + 4 <= C; ++q) *reinterpret_cast<unsigned *>(dst + 4 * q) = src[q];
+            for (int c = 4 * q; c < C; ++c) dst[c] = (signed char)(src[q] >> (8 * (c & 3)));
         }
     }
 }
@@ -812,7 +864,7 @@ static int rows_int8(RowsParams p, cudaStream_t st)
     const bool same = MODE != kNormRes || (offset(p.R, p.ldr) == ox && offset(p.H, p.ldh) == ox);
     const bool odd = ox || p.C % N || p.ldq % N || (reinterpret_cast<uintptr_t>(p.Q) & (N - 1));
     const long long nv = odd ? cdivll((long long)p.C + N - 1, N) : p.C / N;
-    if (!same || nv > 4096) return launch(rows_any_kernel<T, MODE>, dim3((unsigned)p.rows), 512, 0, st, p);
+    if (!same || nv > 4096) return launch(rows_any_kernel<T, MODE, false>, dim3((unsigned)p.rows), 512, 0, st, p);
     // Rows that fit the GPU at once with a thread for every load (1024 threads an SM) are taken so: norm with a shortcut, us in a graph,
     // 300 x 1024 bf16 2.4, the other way 4.4; beyond the bound 2000 x 1283 bf16 10.6 and 8.9, 600 x 1283 float 6.9 and 4.5.  Else a row in a warp or a part of one up to 128 loads, and four
     // or eight loads a thread.
@@ -841,19 +893,20 @@ static int nchw_int8(RowsParams p, cudaStream_t st)
     const long long tiles = cdivll(p.rows, 32);
     // warps that share 32 pixels: as few as the registers allow, more where the pixels are few; blocks of two warps (256 x 64 x 56 x 56: 46.4
     // us; of eight, which wait for the last of them, 50.7; two warps to a tile 48.3)
-    int share = 1;
-    while (share < 16 && words > share * most) share *= 2;
-    while (share < 16 && words >= 4 * share && tiles * share < 8 * kNumSMs) share *= 2;
-    const bool loop = words > share * most || (long long)p.C * p.HW > 0x7fffffffLL;
-    if (loop) share = 16;
+    int share = std::min(16, cdiv(words, most));
+    while (share < 9 && words >= 4 * share && tiles * share < 8 * kNumSMs) share = std::min(16, 2 * share);
+    const bool loop = words > share * most || p.C < 4;          // (128 x 512 x 14 x 14 bf16 so: 27 us, in registers 12)
+    if (loop) share = 8;
     p.group = share;
-    const int warps = std::max(2, share), per_block = warps / share;
+    const int per_block = share == 1 ? 2 : 1, warps = share * per_block;
     const long long blocks = cdivll(tiles, per_block);
     if (blocks > 0x7fffffffLL) return WG2X2_ERR_UNSUPPORTED;
-    const bool by16 = p.C % 16 == 0 && p.ldq % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Q) & 15u) == 0;
-    const int pieces = by16 ? words / 4 : words;
+    const bool by16 = p.ldq % 16 == 0 && (reinterpret_cast<uintptr_t>(p.Q) & 15u) == 0;
+    const int pieces = by16 ? p.C / 16 : words;
     p.inv = pieces > 1 ? (unsigned)((0x100000000ull + pieces - 1) / pieces) : 0;       // i / pieces exact for i * pieces < 2^32
-    const size_t smem = loop ? 0 : (size_t)per_block * 32 * (words | 1) * 4 + (MODE != kQuantize ? (size_t)16 * words : 0);
+    const size_t smem = (size_t)per_block * 32 * (words | 1) * 4 + (MODE != kQuantize ? (size_t)16 * words : 0);
+    if (smem > 216 * 1024)
+        return p.rows > 0x7fffffffLL ? WG2X2_ERR_UNSUPPORTED : launch(rows_any_kernel<T, MODE, true>, dim3((unsigned)p.rows), 512, 0, st, p);
     const int nq = loop ? 0 : cdiv(words, share) <= 2 ? 2 : cdiv(words, share) <= 4 ? 4 : cdiv(words, share) <= 8 ? 8 : 16;
     const bool full = p.C == 4 * nq * share;
 #define WG_NCHW(NQ)                                                                                                          \

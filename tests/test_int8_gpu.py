@@ -179,7 +179,7 @@ def test_norm_of_large_and_small_rows():
 
 
 IMAGES = [(1, 1, 1, 1), (2, 3, 5, 7), (3, 4, 1, 33), (2, 63, 9, 9), (1, 64, 56, 56), (5, 65, 7, 7), (2, 128, 14, 13), (1, 200, 6, 6), (3, 256, 7, 7), (2, 300, 4, 4), (1, 512, 7, 7),
-          (2, 600, 3, 5), (1, 1024, 6, 7), (2, 1025, 3, 3), (1, 2500, 2, 9)]
+          (2, 600, 3, 5), (1, 1024, 6, 7), (2, 1025, 3, 3), (1, 2500, 2, 9), (2, 9001, 1, 3), (7, 375, 32, 30), (40, 64, 28, 28), (9, 616, 21, 20)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
