@@ -333,7 +333,7 @@ __device__ __forceinline__ void reduce_block(float &a, float &ss, float2 *part)
 // boundary in every row.  The aligned pieces that a row touches come to shared memory; there the shortcut is added to them, and every
 // thread then reads its N channels at the offset that the row has.
 template <typename T, int MODE, int V, bool BLOCK, bool ODD, int AHEAD>
-__global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256, !BLOCK && V == 4 ? 3 : 1) rows_kernel(const RowsParams p)
+__global__ void __launch_bounds__(BLOCK ? (V == 1 || (V == 4 && AHEAD == 0) ? 1024 : 512) : 256, !BLOCK && V == 4 ? 3 : 1) rows_kernel(const RowsParams p)
 {
     constexpr int N = 16 / sizeof(T), WORDS = N / 4, STAGES = AHEAD + 1;
     constexpr bool SUM = MODE != kQuantize;
@@ -426,10 +426,17 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 ? 1024 : 512) : 256, !BLOCK &&
             Pack a = {{0, 0, 0, 0}};
             if (ODD) {
                 if (c0 < C) {
-                    const unsigned *word = reinterpret_cast<const unsigned *>(got + v * slot) + mis * (int)sizeof(T) / 4;
-                    unsigned t[5];
+                    // (two loads of 16 bytes and selects: word by word, four lanes at a time met in the same banks)
+                    const Pack s0 = pack_at(got + v * slot), s1 = pack_at(got + v * slot + 1);
+                    const bool one = mis * (int)sizeof(T) & 4, two = mis * (int)sizeof(T) & 8;
+                    unsigned r[7], t[5];
 #pragma unroll
-                    for (int j = 0; j < 5; ++j) t[j] = j < 4 || N == 8 ? word[j] : 0;
+                    for (int j = 0; j < 7; ++j) {
+                        const unsigned here = j < 4 ? s0.w[j & 3] : s1.w[j & 3], next = j < 3 ? s0.w[(j + 1) & 3] : s1.w[(j + 1) & 3];
+                        r[j] = one ? next : here;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 5; ++j) t[j] = two ? r[j + 2] : r[j];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) a.w[j] = N == 8 ? __funnelshift_r(t[j], t[j + 1], 16 * (mis & 1)) : t[j];
                 }
@@ -883,7 +890,10 @@ static int rows_int8(RowsParams p, cudaStream_t st)
         return launch_rows<T, MODE, 4, false, 1>(odd, 256, p, st);
     }
     if (nv <= 2048) return launch_rows<T, MODE, 4, true, 1>(odd, (int)(cdivll(nv, 128) * 32), p, st);
-    return launch_rows<T, MODE, 8, true, 0>(odd, (int)(cdivll(nv, 256) * 32), p, st);
+    // (the longest rows: with a shortcut in 32 bits four loads a thread and tensor, which leave registers for twice the threads: 7000 x 10656
+    // 258 us, eight 366; without one four 105, eight 63)
+    constexpr int MOST = N == 4 && MODE == kNormRes ? 4 : 8;
+    return launch_rows<T, MODE, MOST, true, 0>(odd, (int)(cdivll(nv, 32 * MOST) * 32), p, st);
 }
 
 template <typename T, int MODE>
