@@ -737,7 +737,9 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     if (!Q || !q_scale || !W || !w_scale || !Y || ldq < C || ldw < C || (!nchw && ldy < K)) return WG2X2_ERR_BAD_ARG;
     auto off = [](const void *q, unsigned size) { return (reinterpret_cast<uintptr_t>(q) & (size - 1)) != 0; };
     if (off(Q, 16) || off(W, 16) || ldq % 16 || ldw % 16 || off(q_scale, 4) || off(w_scale, 4) || off(bias, 4) || off(Y, e)) return WG2X2_ERR_BAD_ARG;
-    if (C > kLiMaxC || rows > 0x7fffffffLL - 256 || K > 0x7fffffff - 256 || ldq >= 1LL << 40 || ldw >= 1LL << 40) return WG2X2_ERR_UNSUPPORTED;
+    if (C > kLiMaxC || rows > 0x7fffffffLL - 256 || K > 0x7fffffff - 256 || ldq >= 1LL << 40 || ldw >= 1LL << 40 || ldy >= 1LL << 40 ||
+        rows > (1LL << 60) / K)
+        return WG2X2_ERR_UNSUPPORTED;
     const long long ybytes = nchw ? rows * K * e : (long long)K * e, ypitch = nchw ? 0 : ldy * e, ny = nchw ? 1 : rows;
     auto meets = [&](const void *p, long long ld, long long n, long long count) { return p && rows_overlap(Y, ypitch, ybytes, ny, p, ld, n, count); };
     if (meets(Q, ldq, C, rows) || meets(W, ldw, C, K) || meets(q_scale, 0, 4 * rows, 1) || meets(w_scale, 0, 4LL * K, 1) || meets(bias, 0, 4LL * K, 1))
@@ -768,9 +770,9 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     const void *A = nchw ? Q : W, *Bop = nchw ? W : Q;
     const long long lda = nchw ? ldq : ldw, ldb = nchw ? ldw : ldq;
     if (!make_map_codes(&mapA, A, C, p.lanes, lda, kBlockM) || !make_map_codes(&mapB, Bop, C, p.cols, ldb, b_rows)) return WG2X2_ERR_LAUNCH;
-    // More than half of an SM's shared memory, whatever the tile: two CTAs that share an SM would wait for each other's tensor memory, and
-    // with CTAs of their clusters on other SMs, that wait in turn, without an end
-    const size_t smem = std::max((size_t)other + (size_t)p.stages * stage, (size_t)120 * 1024);
+    // CTAs that wait for one another take all of an SM's shared memory, whatever the tile: sharing an SM with another kernel's or cluster's CTA
+    // that holds tensor memory, and waits in turn for a CTA on an SM where this cluster holds some, they could wait without an end
+    const size_t smem = p.splits > 1 || p.pair ? (size_t)kLiSmem : (size_t)other + (size_t)p.stages * stage;
     if (type == WG2X2_F32) return nchw ? li_launch<true, float>(mapA, mapB, p, pairs, smem, st) : li_launch<false, float>(mapA, mapB, p, pairs, smem, st);
     if (type == WG2X2_F16) return nchw ? li_launch<true, __half>(mapA, mapB, p, pairs, smem, st) : li_launch<false, __half>(mapA, mapB, p, pairs, smem, st);
     return nchw ? li_launch<true, __nv_bfloat16>(mapA, mapB, p, pairs, smem, st) : li_launch<false, __nv_bfloat16>(mapA, mapB, p, pairs, smem, st);

@@ -325,9 +325,9 @@ __device__ __forceinline__ void reduce_block(float &a, float &ss, float2 *part)
 }
 
 // Rows in registers: V loads of 16 bytes a thread and tensor.  BLOCK: a row per block, else blockDim.x / group rows.  A warp has
-// neighbouring pieces of a row, V times 32 of them (or of 8 or 16 lanes).
+// neighbouring pieces of a row, V times 32 of them (or V times 2 to 16, where it has several rows).
 // AHEAD: a block has several rows (or blocks of rows) in turn, and the loads of the next AHEAD of them are on their way to shared memory
-// while it works on one.  Every thread fetches the pieces that it uses itself, so nothing waits for other threads.  (16384 x 4096 bf16 with
+// while it works on one.  Every thread fetches the pieces that it uses itself (but for ODD), so nothing waits for other threads.  (16384 x 4096 bf16 with
 // a shortcut: AHEAD = 1 and V = 4 85 us, AHEAD = 2 90, V = 2 100; the next row in registers instead 130.)
 // ODD: rows that do not begin on 16 bytes, or whose length is not a multiple; x, shortcut and sum have the same offset to a 16-byte
 // boundary in every row.  The aligned pieces that a row touches come to shared memory; there the shortcut is added to them, and every
@@ -592,11 +592,12 @@ __global__ void __launch_bounds__(512) rows_any_kernel(const RowsParams p)
 
 // NCHW: lane = pixel (of any images), so that a load is 32 consecutive values of a plane.  p.group warps share a tile of 32 pixels, each
 // with groups of four neighbouring channels, whose codes are a word: NQ groups a thread (0: any number, read a second time).  As many as
-// registers allow, because a thread has costs of its own per pixel (its image, the divisions, the meeting of its warps).  The words are turned through shared memory and leave as pieces of rows.
+// registers allow, because a thread has costs of its own per pixel (its image, the divisions, the meeting of its warps).  The words are
+// turned through shared memory and leave as pieces of rows.
 template <typename T, int MODE, int NQ, bool FULL>
 __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
 {
-    extern __shared__ unsigned turned_all[];        // [tile of the block][32][pitch], then the weights
+    extern __shared__ __align__(16) unsigned turned_all[];        // [tile of the block][32][pitch], then the weights
     __shared__ float2 part[2][16][32];
     constexpr bool SUM = MODE != kQuantize, COARSE = MODE == kQuantize && sizeof(T) == 2;
     wait_for_previous_kernel(kNumSMs);
@@ -873,8 +874,8 @@ static int rows_int8(RowsParams p, cudaStream_t st)
     const long long nv = odd ? cdivll((long long)p.C + N - 1, N) : p.C / N;
     if (!same || nv > 4096) return launch(rows_any_kernel<T, MODE, false>, dim3((unsigned)p.rows), 512, 0, st, p);
     // Rows that fit the GPU at once with a thread for every load (1024 threads an SM) are taken so: norm with a shortcut, us in a graph,
-    // 300 x 1024 bf16 2.4, the other way 4.4; beyond the bound 2000 x 1283 bf16 10.6 and 8.9, 600 x 1283 float 6.9 and 4.5.  Else a row in a warp or a part of one up to 128 loads, and four
-    // or eight loads a thread.
+    // 300 x 1024 bf16 2.4, the other way 4.4; beyond the bound 2000 x 1283 bf16 10.6 and 8.9, 600 x 1283 float 6.9 and 4.5.  Else a row in a
+    // warp or a part of one up to 128 loads, and four or eight loads a thread.
     const bool little = p.rows * nv <= 1024LL * kNumSMs;
     if (little && nv > 32 && nv <= 1024) return launch_rows<T, MODE, 1, true, 0>(odd, (int)(cdivll(nv, 32) * 32), p, st);
     if (nv <= 128) {
@@ -934,7 +935,8 @@ static int codes_int8(int mode, int type, RowsParams &p, long long B, int HW, in
     p.C = C;
     p.HW = HW;
     if (!p.rows) return WG2X2_OK;
-    if (C > 1 << 30) return WG2X2_ERR_UNSUPPORTED;          // (a channel's index and a step beyond it fit 32 bits)
+    if (C > 1 << 30 || p.rows > 1LL << 36 || p.ldx >= 1LL << 40 || p.ldr >= 1LL << 40 || p.ldh >= 1LL << 40 || p.ldq >= 1LL << 40)
+        return WG2X2_ERR_UNSUPPORTED;          // (a channel's index and a step beyond it fit 32 bits; see also the kernels' launchers)
     const int e = type == WG2X2_F32 ? 4 : 2;
     const bool nchw = layout == WG2X2_NCHW;
     if (!p.X || !p.Q || !p.scale || (mode != kQuantize && !p.Wt) || (mode == kNormRes && (!p.R || !p.H))) return WG2X2_ERR_BAD_ARG;
@@ -943,6 +945,7 @@ static int codes_int8(int mode, int type, RowsParams &p, long long B, int HW, in
     if (off(p.X, e) || off(p.R, e) || off(p.H, e) || off(p.scale, 4) || (p.Wt && off(p.Wt, p.w_f32 ? 4 : e))) return WG2X2_ERR_BAD_ARG;
     // the tensors as rows of bytes (an NCHW one: a single row)
     struct Span { const void *at; long long ld, n; };
+    if (nchw && p.rows > (1LL << 60) / C) return WG2X2_ERR_UNSUPPORTED;
     auto image = [&](const void *q, long long ld) { return nchw ? Span{q, 0, p.rows * C * e} : Span{q, ld * e, (long long)C * e}; };
     auto meet = [&](const Span &a, const Span &b) { return a.at && b.at && rows_overlap(a.at, a.ld, a.n, a.ld ? p.rows : 1, b.at, b.ld, b.n, b.ld ? p.rows : 1); };
     const Span q{p.Q, p.ldq, C}, s{p.scale, 0, 4 * p.rows}, x = image(p.X, p.ldx), r = image(p.R, p.ldr), h = image(p.H, p.ldh);

@@ -181,7 +181,8 @@ def quantize_int8(x, relu=False, layout="NHWC", out=None, scale_out=None):
     and scale = max |x| / 127 of a row, q = x / scale to the nearest whole number (ties to even).  layout="NHWC": x (..., C), rows of a
     common pitch, q (..., C), scale (...); "NCHW": x (B,C,H,W), q (B,H,W,C), scale (B,H,W).  relu: of relu(x).  The weights (K,C) of a
     product go through the same call.  Rows of zeros (or with nothing above 2^-119) have scale 0, rows with NaN or infinity scale NaN.
-    q's rows begin on 16-byte boundaries, so for C off a multiple of 16 it is not contiguous."""
+    q's rows begin on 16-byte boundaries, so for C off a multiple of 16 it is not contiguous.  No gradient is recorded, here and in the
+    two calls below."""
     return _native.quantize_int8(x, relu, _LAYOUTS[layout], out, scale_out)
 
 

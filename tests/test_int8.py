@@ -57,11 +57,13 @@ def test_quantize_limits():
     far = dict(X=1 << 50, Q=1 << 52, scale=1 << 54)
     assert quantize(C=(1 << 30) + 1, ldx=1 << 31, ldq=1 << 31, **far) == UNSUPPORTED
     assert quantize(B=1 << 31, **far) == UNSUPPORTED
+    assert quantize(B=1 << 37, **far) == UNSUPPORTED and quantize(ldx=1 << 40, **far) == UNSUPPORTED
     assert quantize(B=1 << 37, layout=1, C=1, **far) == UNSUPPORTED
 
 
 def test_linear_limits():
     assert linear(C=131072, ldq=131072, ldw=131072, W=1 << 32, Y=1 << 40, w_scale=1 << 41, q_scale=1 << 42, bias=1 << 43) == UNSUPPORTED
+    assert linear(B=1 << 30, K=1 << 30, Q=1 << 45, Y=1 << 50, q_scale=1 << 48, w_scale=1 << 47, bias=1 << 46, ldy=1 << 30) == UNSUPPORTED
     assert linear(B=1 << 31, Q=1 << 45, Y=1 << 50, q_scale=1 << 48, ldq=64) == UNSUPPORTED
 
 
