@@ -327,6 +327,39 @@ def test_leading_shapes_and_nothing():
         assert wg2x2.linear_int8(q, s, w, ws, layout="NCHW").shape == (shape[0], 24, shape[2], shape[3])
 
 
+def test_codes_and_scales_are_ordinary_tensors():
+    """Each outlives the other, can be written, saved and loaded, and used as a constant of a graph"""
+    import io
+    g = _gen("ordinary")
+    x = torch.randn((6, 5, 33), generator=g, device="cuda")
+    q, s = wg2x2.quantize_int8(x)
+    q0, s0 = _codes(x.double())
+    keep = s
+    f = io.BytesIO()
+    torch.save((q, s), f)
+    f.seek(0)
+    q2, s2 = torch.load(f)
+    assert torch.equal(q2, q0) and torch.equal(s2, s0.float())
+    w = _rand_codes(g, 7, 33)
+    one = torch.ones(7, device="cuda")
+    assert torch.equal(wg2x2.linear_int8(q2, s2, w, one), wg2x2.linear_int8(q, s, w, one))
+    q.zero_()
+    assert torch.equal(s, s0.float())
+    s.fill_(2.0)
+    assert int(q.abs().max()) == 0 and not q.requires_grad and s.is_leaf
+    del q, s
+    for _ in range(5):
+        wg2x2.quantize_int8(torch.randn_like(x))
+    torch.cuda.synchronize()
+    assert bool((keep == 2).all())
+    w = torch.randn((5,), generator=g, device="cuda", requires_grad=True)
+    (w * wg2x2.quantize_int8(x)[1].sum(0)).sum().backward()
+    assert torch.allclose(w.grad, s0.float().sum(0))
+    with torch.inference_mode():
+        q, s = wg2x2.quantize_int8(x)
+        assert torch.equal(q, q0)
+
+
 def test_refusals():
     x = torch.randn((6, 32), device="cuda")
     w, ws = wg2x2.quantize_int8(torch.randn((8, 32), device="cuda"))
