@@ -544,87 +544,161 @@ linear_int8_pair_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_c
     }
 }
 
-// A few rows of codes: nothing but the weights' bytes counts, and the set-up of the kernels above (tensor memory, barriers, a cluster's
-// exchange) would take longer than those.  `group` lanes have a row of weights, 16 bytes a load and eight loads on their way, and multiply
-// four codes an instruction.  1, 2, 3, 4 rows against the kernels above, us in a graph: 4096 x 4096 (16.8 MB, 2.6 us of memory) 3.2, 4.4,
-// 6.0, 6.5 / 7.4; 512 x 1000 2.1, 2.6, 3.4, 3.4 / 4.6; 8192 x 8192 (10.2 us) 14.5, 15.1, 16.5, 16.5 / 15.8.  Eight rows: 10.3 / 7.4, 5.2 /
-// 4.7, 37.6 / 16.1 (the codes' loads, one for every two rows of weights).
-constexpr int kLiFewRows = 4;
-struct LiFewParams {
+// The next two kernels are for products so small that the set-up of those above (tensor memory, barriers, a cluster's exchange) takes longer
+// than their work.
+struct LiSmallParams {
     const signed char *Q, *W;
     const float *q_scale, *w_scale, *bias;
     void *Y;
     long long ldq, ldw, ldy;
     int rows, C, K, HW, group, relu;        // HW: 0, or an NCHW result's pixels
 };
-// (NR rows of weights at a time where there are several rows of codes, so that a load of those serves as many products)
-template <int ROWS, int NR, typename T>
-__global__ void __launch_bounds__(128) linear_int8_few_kernel(const LiFewParams p)
+
+// One row of codes: nothing but the weights' bytes counts.  `group` lanes have a row of weights, 16 bytes a load and eight loads on their way,
+// and multiply four codes an instruction.  In a graph, against the kernel for a small product below: 4096 x 4096 (16.8 MB, 2.6 us of memory)
+// 5.2 us / 6.2, 4096 x 1000 2.7 / 3.5, 8192 x 1000 6.2 / 8.7.  Several rows are the other kernel's from two on (4096 x 4096: 7.4 / 6.2).
+template <typename T>
+__global__ void __launch_bounds__(128) linear_int8_row_kernel(const LiSmallParams p)
 {
-    constexpr int AT_ONCE = 8 / NR;
+    constexpr int AT_ONCE = 8;
     wait_for_previous_kernel(8 * kNumSMs);
-    const int at = threadIdx.x & (p.group - 1), k = (int)(((long long)blockIdx.x * 128 + threadIdx.x) / p.group) * NR;
-    const signed char *w[NR], *q[ROWS];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) w[n] = p.W + min(k + n, p.K - 1) * p.ldw;
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) q[r] = p.Q + min(r, p.rows - 1) * p.ldq;
-    int acc[NR][ROWS];
-#pragma unroll
-    for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) acc[n][r] = 0;
+    const int at = threadIdx.x & (p.group - 1), k = (int)(((long long)blockIdx.x * 128 + threadIdx.x) / p.group);
+    const signed char *w = p.W + min(k, p.K - 1) * p.ldw;
+    int acc = 0;
     const int pieces = p.C >> 4;
     for (int i0 = at; i0 < pieces; i0 += AT_ONCE * p.group) {
-        int4 v[AT_ONCE][NR];
+        int4 v[AT_ONCE];
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             const int i = i0 + j * p.group;
-#pragma unroll
-            for (int n = 0; n < NR; ++n) v[j][n] = i < pieces ? *reinterpret_cast<const int4 *>(w[n] + 16LL * i) : make_int4(0, 0, 0, 0);
+            v[j] = i < pieces ? *reinterpret_cast<const int4 *>(w + 16LL * i) : make_int4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
-            const int i = min(i0 + j * p.group, pieces - 1);
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                const int4 x = *reinterpret_cast<const int4 *>(q[r] + 16LL * i);
-#pragma unroll
-                for (int n = 0; n < NR; ++n)
-                    acc[n][r] = __dp4a(v[j][n].x, x.x, __dp4a(v[j][n].y, x.y, __dp4a(v[j][n].z, x.z, __dp4a(v[j][n].w, x.w, acc[n][r]))));
-            }
+            const int4 x = *reinterpret_cast<const int4 *>(p.Q + 16LL * min(i0 + j * p.group, pieces - 1));
+            acc = __dp4a(v[j].x, x.x, __dp4a(v[j].y, x.y, __dp4a(v[j].z, x.z, __dp4a(v[j].w, x.w, acc))));
         }
     }
-    for (int c = 16 * pieces + at; c < p.C; c += p.group)
+    for (int c = 16 * pieces + at; c < p.C; c += p.group) acc += (int)w[c] * (int)p.Q[c];
+    for (int o = p.group >> 1; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (at || k >= p.K) return;
+    static_cast<T *>(p.Y)[k] = li_out<T>(li_value(acc, p.w_scale[k], p.q_scale[0], p.bias ? p.bias[k] : -0.f, p.relu ? 0.f : __uint_as_float(0xff800000u)));
+}
+
+// A small product: straight from registers with the warps' matrix instruction (16 rows of codes x 8 of weights x 32 bytes).  A CTA's eight
+// warps share 16 MT rows of codes and 8 NT of weights, each with every eighth 64 bytes of the contraction, two such pieces loaded at once,
+// and meet in shared memory.  Four lanes have 64 bytes of a row, 16 each; which four of those bytes an instruction calls its k-th is the
+// same for both operands, so that no bytes change places.  li_small has the rule and what it measured.
+__device__ __forceinline__ void mma_s8(int (&d)[4], int a0, int a1, int a2, int a3, int b0, int b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 bytes of a row of C from c on, zeros behind its end
+__device__ __forceinline__ int4 li_piece(const signed char *row, int c, int C)
+{
+    if (c + 16 <= C) return *reinterpret_cast<const int4 *>(row + c);
+    int w[4] = {0, 0, 0, 0};
+    if (c < C)
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
+        for (int j = 0; j < 15; ++j)
+            if (c + j < C) w[j >> 2] |= (int)(unsigned char)row[c + j] << (8 * (j & 3));
+    return make_int4(w[0], w[1], w[2], w[3]);
+}
+__host__ __device__ constexpr int li_small_resident(int mt, int nt) { return 6 - mt - nt / 2; }       // CTAs of an SM, what their registers allow
+template <int MT, int NT, typename T>
+__global__ void __launch_bounds__(256, li_small_resident(MT, NT)) linear_int8_small_kernel(const LiSmallParams p)
+{
+    constexpr int COLS = 8 * NT, AT_ONCE = 2, RESIDENT = li_small_resident(MT, NT);
+    __shared__ int sums[8][16 * MT][COLS + 1];
+    wait_for_previous_kernel(RESIDENT * kNumSMs);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * COLS, row0 = blockIdx.y * 16 * MT, rows = min(p.rows - row0, 16 * MT);
+    const signed char *w[NT], *q[MT][2];
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) acc[n][r] += (int)w[n][c] * (int)q[r][c];
+    for (int n = 0; n < NT; ++n) w[n] = p.W + min(n0 + 8 * n + g, p.K - 1) * p.ldw;
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-            for (int o = p.group >> 1; o; o >>= 1) acc[n][r] += __shfl_xor_sync(0xffffffffu, acc[n][r], o);
-    if (at) return;
-    const float low = p.relu ? 0.f : __uint_as_float(0xff800000u);
+        for (int h = 0; h < 2; ++h) q[m][h] = p.Q + (row0 + min(16 * m + 8 * h + g, rows - 1)) * p.ldq;
+    int acc[MT][NT][4];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        if (k + n >= p.K) break;
-        const float ws = p.w_scale[k + n], b = p.bias ? p.bias[k + n] : -0.f;
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            if (r >= p.rows) break;
-            const long long to = p.HW ? (long long)(r / p.HW) * p.K * p.HW + r % p.HW + (long long)(k + n) * p.HW : r * p.ldy + k + n;
-            static_cast<T *>(p.Y)[to] = li_out<T>(li_value(acc[n][r], ws, p.q_scale[r], b, low));
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[m][n][j] = 0;
+    for (int c0 = 64 * warp; c0 < p.C; c0 += AT_ONCE * 512) {
+        int4 b[AT_ONCE][NT], a[AT_ONCE][MT][2];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int c = c0 + 512 * i + 16 * t;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) b[i][n] = li_piece(w[n], c, p.C);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) a[i][m][h] = li_piece(q[m][h], c, p.C);
         }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int4 x = a[i][m][0], y = a[i][m][1], z = b[i][n];
+                    mma_s8(acc[m][n], x.x, y.x, x.y, y.y, z.x, z.y);
+                    mma_s8(acc[m][n], x.z, y.z, x.w, y.w, z.z, z.w);
+                }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[warp][16 * m + 8 * (j >> 1) + g][8 * n + 2 * t + (j & 1)] = acc[m][n][j];
+    const int col = threadIdx.x % COLS, k = n0 + col;
+    const bool have = k < p.K;
+    const float ws = have ? p.w_scale[k] : 0.f, bias = have && p.bias ? p.bias[k] : -0.f, low = p.relu ? 0.f : __uint_as_float(0xff800000u);
+    __syncthreads();
+    for (int i = threadIdx.x / COLS; i < rows; i += 256 / COLS) {
+        const int r = row0 + i;
+        int sum = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sum += sums[u][i][col];
+        const long long to = p.HW ? (long long)(r / p.HW) * p.K * p.HW + r % p.HW + (long long)k * p.HW : r * p.ldy + k;
+        if (have) static_cast<T *>(p.Y)[to] = li_out<T>(li_value(sum, ws, p.q_scale[r], bias, low));
     }
 }
-template <typename T>
-static int li_few(LiFewParams p, cudaStream_t st)
+// Which kernel a product is small enough for: 0 none of the two, 1 the one for a row, 2 to 4 linear_int8_small_kernel with (MT, NT) = (1, 1),
+// (1, 2), (2, 1).  Its CTAs all run at once, and the contraction is short enough that the loads of eight warps hide its latency: up to 16 rows
+// 6144 codes, more rows 4096, and as many CTAs of those as read 1.2 MB of either (each reads all its codes again, from L2).  Against the
+// tensor-memory kernels, us in a graph, rows x C x K: 4 x 512 x 1000 2.1 / 3.9, 16 x 1024 x 4096 2.8 / 4.9, 16 x 2048 x 8192 6.4 / 7.1, 16 x
+// 4096 x 4096 6.6 / 8.0, 16 x 6000 x 6000 10.9 / 11.8; 32 x 64 x 100 2.1 / 4.1, 32 x 512 x 4096 3.5 / 4.4, 32 x 4096 x 2048 7.2 / 7.6, 128 x
+// 1024 x 512 3.0 / 5.2, 128 x 2048 x 1000 5.9 / 6.9, 256 x 512 x 512 3.7 / 4.4.  Behind the rule: 16 x 8192 x 4096 10.8 / 10.5, 16 x 2048 x
+// 12000 8.3 / 7.8, 32 x 4096 x 8192 12.5 / 10.2, 128 x 4096 x 1000 9.4 / 7.8, 256 x 512 x 1000 4.9 / 4.4 (1.0 of the CTAs); 4 x 8192 x 4096
+// 10.5 behind the rule.  One row where the weights' rows are short: 512 x 8192 3.0 / 4.4, 1024 x 4096 2.6 / 2.8; else as above.
+static int li_small(long long rows, int C, int K)
 {
-    for (p.group = 4; p.group < 32 && p.group * 16 < p.C;) p.group *= 2;
-    auto *kernel = p.rows == 1 ? linear_int8_few_kernel<1, 1, T> : p.rows == 2 ? linear_int8_few_kernel<2, 2, T> : linear_int8_few_kernel<4, 2, T>;
-    return launch(kernel, dim3((unsigned)cdivll(p.K, 128 / p.group * (p.rows == 1 ? 1 : 2))), 128, 0, st, p);
+    if (rows == 1 && C > 1024) return 1;
+    if (rows <= 16) {
+        const int ctas = cdiv(K, 8);
+        if (C <= 6144 && ctas <= kNumSMs * li_small_resident(1, 1)) return 2;
+        if (C <= 6144 && cdiv(ctas, 2) <= kNumSMs * li_small_resident(1, 2)) return 3;
+        return rows == 1;
+    }
+    const long long ctas = cdivll(rows, 32) * cdiv(K, 8), most = kNumSMs * li_small_resident(2, 1);
+    return C <= 4096 && ctas <= most && ctas * C <= 2048 * most ? 4 : 0;
+}
+template <typename T>
+static int li_launch_small(int which, LiSmallParams p, cudaStream_t st)
+{
+    if (which == 1) {
+        for (p.group = 4; p.group < 32 && p.group * 16 < p.C;) p.group *= 2;
+        return launch(linear_int8_row_kernel<T>, dim3((unsigned)cdivll(p.K, 128 / p.group)), 128, 0, st, p);
+    }
+    auto *kernel = which == 2 ? linear_int8_small_kernel<1, 1, T> : which == 3 ? linear_int8_small_kernel<1, 2, T> : linear_int8_small_kernel<2, 1, T>;
+    return launch(kernel, dim3((unsigned)cdiv(p.K, which == 3 ? 16 : 8), (unsigned)cdiv(p.rows, 32)), 256, 0, st, p);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -744,12 +818,12 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     auto meets = [&](const void *p, long long ld, long long n, long long count) { return p && rows_overlap(Y, ypitch, ybytes, ny, p, ld, n, count); };
     if (meets(Q, ldq, C, rows) || meets(W, ldw, C, K) || meets(q_scale, 0, 4 * rows, 1) || meets(w_scale, 0, 4LL * K, 1) || meets(bias, 0, 4LL * K, 1))
         return WG2X2_ERR_BAD_ARG;
-    if (rows <= kLiFewRows) {
-        LiFewParams f = {};
+    if (const int which = li_small(rows, C, K)) {
+        LiSmallParams f = {};
         f.Q = static_cast<const signed char *>(Q); f.W = static_cast<const signed char *>(W);
         f.q_scale = q_scale; f.w_scale = w_scale; f.bias = bias; f.Y = Y; f.ldq = ldq; f.ldw = ldw; f.ldy = ldy;
         f.rows = (int)rows; f.C = C; f.K = K; f.HW = nchw ? HW : 0; f.relu = relu != 0;
-        return type == WG2X2_F32 ? li_few<float>(f, st) : type == WG2X2_F16 ? li_few<__half>(f, st) : li_few<__nv_bfloat16>(f, st);
+        return type == WG2X2_F32 ? li_launch_small<float>(which, f, st) : type == WG2X2_F16 ? li_launch_small<__half>(which, f, st) : li_launch_small<__nv_bfloat16>(which, f, st);
     }
     LiParams p = {};
     p.Y = Y; p.ldy = ldy; p.bias = bias; p.K = K; p.HW = HW; p.relu = relu != 0;
