@@ -556,7 +556,7 @@ struct LiSmallParams {
 
 // One row of codes: nothing but the weights' bytes counts.  `group` lanes have a row of weights, 16 bytes a load and eight loads on their way,
 // and multiply four codes an instruction.  In a graph, against the kernel for a small product below: 4096 x 4096 (16.8 MB, 2.6 us of memory)
-// 5.2 us / 6.2, 4096 x 1000 2.7 / 3.5, 8192 x 1000 6.2 / 8.7.  Several rows are the other kernel's from two on (4096 x 4096: 7.4 / 6.2).
+// 5.1 us / 5.6, 4096 x 1000 2.6 / 3.2, 8192 x 4096 8.0 / 9.6.  Several rows are the other kernel's from two on (4096 x 4096: 7.4 / 5.6).
 template <typename T>
 __global__ void __launch_bounds__(128) linear_int8_row_kernel(const LiSmallParams p)
 {
@@ -585,10 +585,10 @@ __global__ void __launch_bounds__(128) linear_int8_row_kernel(const LiSmallParam
     static_cast<T *>(p.Y)[k] = li_out<T>(li_value(acc, p.w_scale[k], p.q_scale[0], p.bias ? p.bias[k] : -0.f, p.relu ? 0.f : __uint_as_float(0xff800000u)));
 }
 
-// A small product: straight from registers with the warps' matrix instruction (16 rows of codes x 8 of weights x 32 bytes).  A CTA's eight
-// warps share 16 MT rows of codes and 8 NT of weights, each with every eighth 64 bytes of the contraction, two such pieces loaded at once,
-// and meet in shared memory.  Four lanes have 64 bytes of a row, 16 each; which four of those bytes an instruction calls its k-th is the
-// same for both operands, so that no bytes change places.  li_small has the rule and what it measured.
+// A small product: straight from registers with the warps' matrix instruction (16 x 8 rows, 32 bytes of both).  A CTA has 16 TILES rows of
+// codes and 8 of weights (CODES16), or 8 TILES of codes and 16 of weights.  Its eight warps take every eighth 64 bytes of the contraction
+// each, AT_ONCE such pieces loaded at once, and meet in shared memory.  Four lanes have 64 bytes of a row, 16 each; which four of those bytes
+// an instruction calls its k-th is the same for both operands, so that no bytes change places.  li_small has the rule and what it measured.
 __device__ __forceinline__ void mma_s8(int (&d)[4], int a0, int a1, int a2, int a3, int b0, int b1)
 {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -605,22 +605,23 @@ __device__ __forceinline__ int4 li_piece(const signed char *row, int c, int C)
             if (c + j < C) w[j >> 2] |= (int)(unsigned char)row[c + j] << (8 * (j & 3));
     return make_int4(w[0], w[1], w[2], w[3]);
 }
-__host__ __device__ constexpr int li_small_resident(int mt, int nt) { return 6 - mt - nt / 2; }       // CTAs of an SM, what their registers allow
-template <int MT, int NT, typename T>
-__global__ void __launch_bounds__(256, li_small_resident(MT, NT)) linear_int8_small_kernel(const LiSmallParams p)
+template <bool CODES16, int TILES, int AT_ONCE, int RESIDENT, typename T>
+__global__ void __launch_bounds__(256, RESIDENT) linear_int8_small_kernel(const LiSmallParams p)
 {
-    constexpr int COLS = 8 * NT, AT_ONCE = 2, RESIDENT = li_small_resident(MT, NT);
-    __shared__ int sums[8][16 * MT][COLS + 1];
+    constexpr int MT = CODES16 ? TILES : 1, NT = CODES16 ? 1 : TILES, ROWS = CODES16 ? 16 * MT : 8 * NT, COLS = CODES16 ? 8 : 16;
+    __shared__ int sums[8][ROWS][COLS + 1];
     wait_for_previous_kernel(RESIDENT * kNumSMs);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * COLS, row0 = blockIdx.y * 16 * MT, rows = min(p.rows - row0, 16 * MT);
-    const signed char *w[NT], *q[MT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) w[n] = p.W + min(n0 + 8 * n + g, p.K - 1) * p.ldw;
+    const int n0 = blockIdx.x * COLS, row0 = blockIdx.y * ROWS, rows = min(p.rows - row0, ROWS);
+    auto codes = [&](int i) { return p.Q + (row0 + min(i + g, rows - 1)) * p.ldq; };
+    auto weights = [&](int i) { return p.W + min(n0 + i + g, p.K - 1) * p.ldw; };
+    const signed char *pa[MT][2], *pb[NT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) q[m][h] = p.Q + (row0 + min(16 * m + 8 * h + g, rows - 1)) * p.ldq;
+        for (int h = 0; h < 2; ++h) pa[m][h] = CODES16 ? codes(16 * m + 8 * h) : weights(16 * m + 8 * h);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) pb[n] = CODES16 ? weights(8 * n) : codes(8 * n);
     int acc[MT][NT][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -629,16 +630,16 @@ __global__ void __launch_bounds__(256, li_small_resident(MT, NT)) linear_int8_sm
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[m][n][j] = 0;
     for (int c0 = 64 * warp; c0 < p.C; c0 += AT_ONCE * 512) {
-        int4 b[AT_ONCE][NT], a[AT_ONCE][MT][2];
+        int4 a[AT_ONCE][MT][2], b[AT_ONCE][NT];
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
             const int c = c0 + 512 * i + 16 * t;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) b[i][n] = li_piece(w[n], c, p.C);
-#pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) a[i][m][h] = li_piece(q[m][h], c, p.C);
+                for (int h = 0; h < 2; ++h) a[i][m][h] = li_piece(pa[m][h], c, p.C);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) b[i][n] = li_piece(pb[n], c, p.C);
         }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i)
@@ -656,7 +657,10 @@ __global__ void __launch_bounds__(256, li_small_resident(MT, NT)) linear_int8_sm
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sums[warp][16 * m + 8 * (j >> 1) + g][8 * n + 2 * t + (j & 1)] = acc[m][n][j];
+            for (int j = 0; j < 4; ++j) {
+                const int ia = 16 * m + 8 * (j >> 1) + g, ib = 8 * n + 2 * t + (j & 1);
+                sums[warp][CODES16 ? ia : ib][CODES16 ? ib : ia] = acc[m][n][j];
+            }
     const int col = threadIdx.x % COLS, k = n0 + col;
     const bool have = k < p.K;
     const float ws = have ? p.w_scale[k] : 0.f, bias = have && p.bias ? p.bias[k] : -0.f, low = p.relu ? 0.f : __uint_as_float(0xff800000u);
@@ -670,35 +674,45 @@ __global__ void __launch_bounds__(256, li_small_resident(MT, NT)) linear_int8_sm
         if (have) static_cast<T *>(p.Y)[to] = li_out<T>(li_value(sum, ws, p.q_scale[r], bias, low));
     }
 }
-// Which kernel a product is small enough for: 0 none of the two, 1 the one for a row, 2 to 4 linear_int8_small_kernel with (MT, NT) = (1, 1),
-// (1, 2), (2, 1).  Its CTAs all run at once, and the contraction is short enough that the loads of eight warps hide its latency: up to 16 rows
-// 6144 codes, more rows 4096, and as many CTAs of those as read 1.2 MB of either (each reads all its codes again, from L2).  Against the
-// tensor-memory kernels, us in a graph, rows x C x K: 4 x 512 x 1000 2.1 / 3.9, 16 x 1024 x 4096 2.8 / 4.9, 16 x 2048 x 8192 6.4 / 7.1, 16 x
-// 4096 x 4096 6.6 / 8.0, 16 x 6000 x 6000 10.9 / 11.8; 32 x 64 x 100 2.1 / 4.1, 32 x 512 x 4096 3.5 / 4.4, 32 x 4096 x 2048 7.2 / 7.6, 128 x
-// 1024 x 512 3.0 / 5.2, 128 x 2048 x 1000 5.9 / 6.9, 256 x 512 x 512 3.7 / 4.4.  Behind the rule: 16 x 8192 x 4096 10.8 / 10.5, 16 x 2048 x
-// 12000 8.3 / 7.8, 32 x 4096 x 8192 12.5 / 10.2, 128 x 4096 x 1000 9.4 / 7.8, 256 x 512 x 1000 4.9 / 4.4 (1.0 of the CTAs); 4 x 8192 x 4096
-// 10.5 behind the rule.  One row where the weights' rows are short: 512 x 8192 3.0 / 4.4, 1024 x 4096 2.6 / 2.8; else as above.
-static int li_small(long long rows, int C, int K)
+template <bool CODES16, int TILES, int AT_ONCE, int RESIDENT, typename T>
+static bool li_small_launch(const LiSmallParams &p, cudaStream_t st, int *rc)
 {
-    if (rows == 1 && C > 1024) return 1;
-    if (rows <= 16) {
-        const int ctas = cdiv(K, 8);
-        if (C <= 6144 && ctas <= kNumSMs * li_small_resident(1, 1)) return 2;
-        if (C <= 6144 && cdiv(ctas, 2) <= kNumSMs * li_small_resident(1, 2)) return 3;
-        return rows == 1;
-    }
-    const long long ctas = cdivll(rows, 32) * cdiv(K, 8), most = kNumSMs * li_small_resident(2, 1);
-    return C <= 4096 && ctas <= most && ctas * C <= 2048 * most ? 4 : 0;
+    const long long across = cdiv(p.K, CODES16 ? 8 : 16), down = cdiv(p.rows, CODES16 ? 16 * TILES : 8 * TILES);
+    if (across * down > RESIDENT * kNumSMs) return false;
+    *rc = launch(linear_int8_small_kernel<CODES16, TILES, AT_ONCE, RESIDENT, T>, dim3((unsigned)across, (unsigned)down), 256, 0, st, p);
+    return true;
 }
+// Launches a product that is small enough for one of the two, or says that it is not.  The CTAs of the second all run at once (in two waves
+// they would load their codes twice over and lose), and the contraction is short enough for the loads of eight warps.  Against the kernels
+// with tensor memory, us in a graph, rows x C x K (weights in turn, 250 MB of them or 16 sets):
+//    up to 8 rows: the instruction's narrow side, half as many loads of codes.  8 x 512 x 1000 1.9 / 3.7, 8 x 1024 x 4096 2.3 / 4.9, 8 x 2048 x
+//       8191 5.4 / 7.0, 8 x 4096 x 4096 5.8 / 8.1, 8 x 8192 x 4096 9.9 / 10.6; behind the rule 8 x 4096 x 12000 12.3 / 10.9.  Four pieces at
+//       once where there are that many: 8 x 4096 x 4096 6.5 with two
+//    9 to 16: 16 x 512 x 1000 2.1 / 3.7, 16 x 1024 x 4096 2.7 / 4.9, 16 x 4096 x 4096 6.6 / 8.1; behind it 16 x 6100 x 1000 7.8 / 6.7, 16 x 4096
+//       x 12000 13.0 / 10.9.  With more than 740 CTAs of eight rows of weights, sixteen: 16 x 2048 x 8191 6.4 / 7.0
+//    more: 32 x 64 x 100 2.1 / 3.9, 32 x 512 x 4096 3.3 / 4.4, 32 x 4096 x 4096 8.5 / 9.6, 128 x 2048 x 1000 4.8 / 6.8, 128 x 4096 x 1000 7.7 /
+//       8.0; behind it 32 x 2048 x 8191 8.8 / 7.5, 256 x 512 x 1000 5.0 / 4.4.  32 x 16 rows a CTA where that is one for nearly every SM, else 32
+//       x 8: 32 x 512 x 1000 2.6 / 2.8 with the wide ones, 32 x 2048 x 4096 5.7 / 6.3 with the narrow
+//    one row: see above; in short rows of weights the second kernel is the faster too (1 x 512 x 8191 2.4 / 4.4, 1 x 1024 x 4096 2.3 / 2.8)
 template <typename T>
-static int li_launch_small(int which, LiSmallParams p, cudaStream_t st)
+static bool li_small(LiSmallParams p, long long rows, cudaStream_t st, int *rc)
 {
-    if (which == 1) {
-        for (p.group = 4; p.group < 32 && p.group * 16 < p.C;) p.group *= 2;
-        return launch(linear_int8_row_kernel<T>, dim3((unsigned)cdivll(p.K, 128 / p.group)), 128, 0, st, p);
+    const int C = p.C;
+    if (rows > 32 * 4 * kNumSMs) return false;
+    p.rows = (int)rows;
+    if (rows == 1 && C > 1024) {
+    } else if (rows <= 8) {
+        if (C <= 1024 && li_small_launch<false, 1, 2, 5, T>(p, st, rc)) return true;
+        if (C > 1024 && C <= 8192 && li_small_launch<false, 1, 4, 4, T>(p, st, rc)) return true;
+    } else if (rows <= 16) {
+        if (C <= 4096 && (li_small_launch<true, 1, 2, 5, T>(p, st, rc) || li_small_launch<false, 2, 2, 4, T>(p, st, rc))) return true;
+    } else if (C <= 4096) {
+        return cdivll(rows, 32) * cdiv(p.K, 16) < 128 ? li_small_launch<true, 2, 2, 4, T>(p, st, rc) : li_small_launch<false, 4, 2, 2, T>(p, st, rc);
     }
-    auto *kernel = which == 2 ? linear_int8_small_kernel<1, 1, T> : which == 3 ? linear_int8_small_kernel<1, 2, T> : linear_int8_small_kernel<2, 1, T>;
-    return launch(kernel, dim3((unsigned)cdiv(p.K, which == 3 ? 16 : 8), (unsigned)cdiv(p.rows, 32)), 256, 0, st, p);
+    if (rows > 1) return false;
+    for (p.group = 4; p.group < 32 && p.group * 16 < C;) p.group *= 2;
+    *rc = launch(linear_int8_row_kernel<T>, dim3((unsigned)cdivll(p.K, 128 / p.group)), 128, 0, st, p);
+    return true;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -818,13 +832,12 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     auto meets = [&](const void *p, long long ld, long long n, long long count) { return p && rows_overlap(Y, ypitch, ybytes, ny, p, ld, n, count); };
     if (meets(Q, ldq, C, rows) || meets(W, ldw, C, K) || meets(q_scale, 0, 4 * rows, 1) || meets(w_scale, 0, 4LL * K, 1) || meets(bias, 0, 4LL * K, 1))
         return WG2X2_ERR_BAD_ARG;
-    if (const int which = li_small(rows, C, K)) {
-        LiSmallParams f = {};
-        f.Q = static_cast<const signed char *>(Q); f.W = static_cast<const signed char *>(W);
-        f.q_scale = q_scale; f.w_scale = w_scale; f.bias = bias; f.Y = Y; f.ldq = ldq; f.ldw = ldw; f.ldy = ldy;
-        f.rows = (int)rows; f.C = C; f.K = K; f.HW = nchw ? HW : 0; f.relu = relu != 0;
-        return type == WG2X2_F32 ? li_launch_small<float>(which, f, st) : type == WG2X2_F16 ? li_launch_small<__half>(which, f, st) : li_launch_small<__nv_bfloat16>(which, f, st);
-    }
+    LiSmallParams f = {};
+    f.Q = static_cast<const signed char *>(Q); f.W = static_cast<const signed char *>(W);
+    f.q_scale = q_scale; f.w_scale = w_scale; f.bias = bias; f.Y = Y; f.ldq = ldq; f.ldw = ldw; f.ldy = ldy;
+    f.C = C; f.K = K; f.HW = nchw ? HW : 0; f.relu = relu != 0;
+    int rc;
+    if (type == WG2X2_F32 ? li_small<float>(f, rows, st, &rc) : type == WG2X2_F16 ? li_small<__half>(f, rows, st, &rc) : li_small<__nv_bfloat16>(f, rows, st, &rc)) return rc;
     LiParams p = {};
     p.Y = Y; p.ldy = ldy; p.bias = bias; p.K = K; p.HW = HW; p.relu = relu != 0;
     p.lane_scale = nchw ? q_scale : w_scale;

@@ -240,8 +240,10 @@ LINEAR = [(1, 1, 1), (4, 15, 9), (4, 31, 100), (2, 500, 700), (3, 129, 33), (4, 
           # small products, up to the limits, and those just behind them
           (16, 6144, 700), (9, 64, 5920), (9, 65, 5921), (15, 70, 9472), (16, 100, 9473), (2, 6145, 9), (6, 2000, 6001), (256, 512, 512), (40, 33, 2368), (64, 1030, 2369),
           (1, 600, 9000), (1, 64, 20000), (1, 1025, 9), (2300, 24, 65), (32, 4096, 2048), (32, 4096, 2400), (17, 4097, 31), (129, 4080, 370),
+          (8, 64, 11840), (7, 70, 11841), (8, 1025, 9472), (5, 1030, 9473), (8, 8192, 100), (8, 8193, 100), (16, 4096, 300), (16, 4097, 300), (10, 130, 5921), (24, 900, 4736), (32, 2049, 4737), (288, 600, 500),
+          (17, 100, 2032), (17, 100, 2033), (130, 3000, 400),
           # clusters that share a tile: few rows and long contractions
-          (3, 9000, 40), (5, 8192, 128), (7, 7001, 1000), (16, 6200, 333), (31, 8000, 257), (33, 5000, 127), (64, 4500, 100), (127, 4224, 128),
+          (3, 9000, 40), (5, 8192, 128), (7, 7001, 1000), (16, 6200, 333), (31, 8000, 257), (33, 5000, 127), (64, 4500, 100), (127, 4224, 128), (6, 8200, 333), (9, 8192, 128),
           # tiles of 256 x 256 and 256 x 128 on pairs of SMs, ragged
           (4100, 700, 3001), (3000, 1024, 2048), (8192, 300, 4097), (2600, 2000, 5000), (700, 4100, 9000)]
 
@@ -262,7 +264,7 @@ def test_linear(rows, C, K):
         _check_linear(y, want, p, dtype)
 
 
-@pytest.mark.parametrize("B,H,W,C,K", [(1, 1, 1, 5, 3), (2, 1, 2, 100, 7), (1, 1, 3, 512, 1000), (1, 7, 7, 512, 100), (2, 7, 7, 64, 64), (1, 7, 7, 5000, 100), (3, 5, 9, 4130, 33), (1, 1, 3, 7000, 1000), (2, 2, 3, 200, 6000), (5, 1, 3, 72, 40), (3, 5, 9, 130, 33), (4, 28, 28, 64, 128), (1, 56, 56, 64, 64), (40, 14, 14, 128, 256),
+@pytest.mark.parametrize("B,H,W,C,K", [(1, 1, 1, 5, 3), (2, 1, 2, 100, 7), (1, 1, 3, 512, 1000), (1, 7, 7, 512, 100), (2, 7, 7, 64, 64), (1, 7, 7, 5000, 100), (3, 5, 9, 4130, 33), (1, 1, 3, 7000, 1000), (1, 1, 3, 9000, 1000), (3, 4, 5, 500, 2100), (2, 2, 3, 200, 6000), (5, 1, 3, 72, 40), (3, 5, 9, 130, 33), (4, 28, 28, 64, 128), (1, 56, 56, 64, 64), (40, 14, 14, 128, 256),
                                        (64, 7, 7, 256, 512), (2, 1, 130, 2000, 17), (30, 28, 27, 33, 300), (64, 14, 14, 600, 1030), (17, 28, 28, 1024, 513)])
 def test_linear_images(B, H, W, C, K):
     g = _gen("li", B, H, W, C, K)
@@ -466,7 +468,7 @@ def test_streams_threads_and_graphs():
 def test_shared_tiles_on_several_streams():
     """Products whose tiles are shared by clusters, many of them at once: no two wait for each other"""
     g = _gen("several")
-    shapes = [(8, 1024, 256), (16, 4096, 128), (40, 2048, 512), (100, 8192, 1024), (9, 640, 64), (8, 8192, 256), (16, 10000, 128), (40, 8192, 512)]
+    shapes = [(8, 1024, 256), (16, 4096, 128), (40, 2048, 512), (100, 8192, 1024), (9, 640, 64), (9, 8192, 256), (16, 10000, 128), (40, 8192, 512)]
     sets = []
     for rows, C, K in shapes:
         q, w = _rand_codes(g, rows, C), _rand_codes(g, K, C)
