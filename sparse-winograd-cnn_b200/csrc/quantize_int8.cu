@@ -851,7 +851,10 @@ static int launch_rows(int threads, const RowsParams &p, cudaStream_t st)
             cudaFuncAttributes a;
             return cudaFuncGetAttributes(&a, reinterpret_cast<const void *>(kernel)) == cudaSuccess && a.numRegs > 0 ? (a.numRegs + 7) / 8 * 8 : 128;
         }();
-        const long long at_once = std::max(1, std::min({2048 / threads, 65536 / (regs * threads), (int)(228 * 1024 / (smem + 2048))}));
+        // (a quarter of the SM's registers for every fourth warp: five blocks of three warps with 112 registers, not six, the last of which
+        // would begin when others have ended)
+        const int warps = threads / 32, by_regs = 16384 / (regs * 32) * 4 / warps;
+        const long long at_once = std::max(1, std::min({64 / warps, by_regs, (int)(228 * 1024 / (smem + 2048))}));
         blocks = std::min(blocks, kNumSMs * at_once);
     }
     return launch(kernel, dim3((unsigned)blocks), threads, smem, st, p);
