@@ -346,11 +346,6 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 || (V == 4 && AHEAD == 0) ? 10
     const int width = BLOCK ? 32 : p.group, at = lane & (width - 1);
     const int i0 = BLOCK ? (threadIdx.x >> 5) * (32 * V) + lane : at;           // the thread's pieces: i0 + v * width
     const int per_block = BLOCK ? 1 : blockDim.x / p.group, mine = BLOCK ? 0 : threadIdx.x / p.group;
-    // Loads of which no lane of the group has a value: unaligned rows touch a piece more than their length has, and where that is one above a
-    // power of two half the loads are such (200000 x 63 float 31 us, left out 28; 65536 x 255 bf16 28.6, 24.3).  Not in the others: the branches
-    // keep the loads from one another (16384 x 4096 float, aligned, 51 us, with them 56; a block a row 71, 76; with a shortcut 54, 58).
-    constexpr bool LEAVE_OUT = ODD && MODE == kQuantize && !BLOCK && V == 4;
-    auto behind = [&](int v) { return LEAVE_OUT && v * width * N >= p.C; };
     const long long stride = (long long)gridDim.x * per_block, first = (long long)blockIdx.x * per_block;
     const float low = p.relu ? 0.f : __uint_as_float(0xff800000u);
     const T *X = static_cast<const T *>(p.X), *R = static_cast<const T *>(p.R);
@@ -427,7 +422,6 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 || (V == 4 && AHEAD == 0) ? 10
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if (behind(v)) continue;
             const int c0 = (i0 + v * width) * N;
             Pack a = {{0, 0, 0, 0}};
             if (ODD) {
@@ -469,7 +463,6 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 || (V == 4 && AHEAD == 0) ? 10
         float amax = 0.f, ss = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if (behind(v)) continue;
             if (MODE != kQuantize) {
                 float w[N];
                 if (W_AT_HAND) {
@@ -525,7 +518,6 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 || (V == 4 && AHEAD == 0) ? 10
         unsigned w[V][WORDS];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if (behind(v)) continue;
             code_words<N, MODE == kQuantize && N == 8>(u[v], k.inv, k.a, w[v]);
 #pragma unroll
             for (int g = 0; g < WORDS; ++g) w[v][g] &= k.live;
