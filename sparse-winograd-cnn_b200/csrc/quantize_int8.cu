@@ -331,7 +331,9 @@ __device__ __forceinline__ void reduce_block(float &a, float &ss, float2 *part)
 // a shortcut: AHEAD = 1 and V = 4 85 us, AHEAD = 2 90, V = 2 100; the next row in registers instead 130.)
 // ODD: rows that do not begin on 16 bytes, or whose length is not a multiple; x, shortcut and sum have the same offset to a 16-byte
 // boundary in every row.  The aligned pieces that a row touches come to shared memory; there the shortcut is added to them, and every
-// thread then reads its N channels at the offset that the row has.
+// thread then reads its N channels at the offset that the row has.  A row can touch a piece more than its length has; the thread of its first
+// channels fetches that one too (a load slot for it left half of the slots empty
+// where the length is just below a power of two: 65536 x 255 float 40 us, now 24, 8192 x 4095 with a shortcut 117, 88).
 template <typename T, int MODE, int V, bool BLOCK, bool ODD, int AHEAD>
 __global__ void __launch_bounds__(BLOCK ? (V == 1 || (V == 4 && AHEAD == 0) ? 1024 : 512) : 256, !BLOCK && V == 4 ? 3 : 1) rows_kernel(const RowsParams p)
 {
@@ -375,6 +377,11 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 || (V == 4 && AHEAD == 0) ? 10
                 fetch_pack<T, N>(ring + o, ring_at + 16u * o, xf, c0, p.C, safe, X, x_end);
                 if (MODE == kNormRes) fetch_pack<T, N>(ring + o + half, ring_at + 16u * (o + half), rf, c0, p.C, safe, R, r_end);
             }
+            if (ODD && i0 == 0) {
+                const int c0 = in_row * N - mis, o = at0 + in_row;
+                fetch_pack<T, N>(ring + o, ring_at + 16u * o, xf, c0, p.C, safe, X, x_end);
+                if (MODE == kNormRes) fetch_pack<T, N>(ring + o + half, ring_at + 16u * (o + half), rf, c0, p.C, safe, R, r_end);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         next += stride;
@@ -408,14 +415,15 @@ __global__ void __launch_bounds__(BLOCK ? (V == 1 || (V == 4 && AHEAD == 0) ? 10
         uint4 *const got = ring + get * stage + mine_in;
         if (ODD) {
             if (MODE == kNormRes) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const int c0 = (i0 + v * width) * N - mis;
-                    if (c0 >= C) continue;
-                    const Pack sum = Types<T>::sum(pack_at(got + v * slot), pack_at(got + v * slot + half));
+                auto add = [&](uint4 *piece, int c0) {
+                    if (c0 >= C) return;
+                    const Pack sum = Types<T>::sum(pack_at(piece), pack_at(piece + half));
                     store_pack<T, N, true>(h, c0, C, sum);
-                    got[v * slot] = make_uint4(sum.w[0], sum.w[1], sum.w[2], sum.w[3]);
-                }
+                    *piece = make_uint4(sum.w[0], sum.w[1], sum.w[2], sum.w[3]);
+                };
+#pragma unroll
+                for (int v = 0; v < V; ++v) add(got + v * slot, (i0 + v * width) * N - mis);
+                if (i0 == 0) add(got + in_row, in_row * N - mis);
             }
             if (BLOCK) __syncthreads();
             else __syncwarp();
@@ -874,7 +882,7 @@ static int rows_int8(RowsParams p, cudaStream_t st)
     const unsigned ox = offset(p.X, p.ldx);
     const bool same = MODE != kNormRes || (offset(p.R, p.ldr) == ox && offset(p.H, p.ldh) == ox);
     const bool odd = ox || p.C % N || p.ldq % N || (reinterpret_cast<uintptr_t>(p.Q) & (N - 1));
-    const long long nv = odd ? cdivll((long long)p.C + N - 1, N) : p.C / N;
+    const long long nv = cdivll(p.C, N);
     if (!same || nv > 4096) return launch(rows_any_kernel<T, MODE, false>, dim3((unsigned)p.rows), 512, 0, st, p);
     // Rows that fit the GPU at once with a thread for every load (1024 threads an SM) are taken so: norm with a shortcut, us in a graph,
     // 300 x 1024 bf16 2.4, the other way 4.4; beyond the bound 2000 x 1283 bf16 10.6 and 8.9, 600 x 1283 float 6.9 and 4.5.  Else a row in a
