@@ -924,6 +924,30 @@ PyObject *py_linear_int8(WG_ARGS)
     END_HANDLE_TH_ERRORS
 }
 
+// weights (a tuple of tensors), seen (for each: the tensor, a tensor of its memory, its address, its version) -> whether they still are what was seen: the
+// same tensors over the same memory, and nothing has been written to them that torch counts.  (Native: a network asks for some thirty
+// weights a pass.)
+PyObject *py_unchanged(WG_ARGS)
+{
+    HANDLE_TH_ERRORS
+    want(n, 2);
+    if (!PyTuple_Check(a[0]) || !PyTuple_Check(a[1])) type_error("weights and what was seen of them must be tuples");
+    if (PyTuple_GET_SIZE(a[0]) != PyTuple_GET_SIZE(a[1])) Py_RETURN_FALSE;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[0]); ++i) {
+        PyObject *w = PyTuple_GET_ITEM(a[0], i), *s = PyTuple_GET_ITEM(a[1], i);
+        if (!THPVariable_Check(w) || !PyTuple_Check(s) || PyTuple_GET_SIZE(s) != 4) type_error("weights must be tensors, each with what was seen of it");
+        if (w != PyTuple_GET_ITEM(s, 0)) Py_RETURN_FALSE;
+        const Tensor &t = THPVariable_Unpack(w);
+        if (t.is_inference()) Py_RETURN_FALSE;              // (torch counts no writes to such a tensor)
+        const void *at = PyLong_AsVoidPtr(PyTuple_GET_ITEM(s, 2));
+        const long version = PyLong_AsLong(PyTuple_GET_ITEM(s, 3));
+        if (PyErr_Occurred()) throw python_error();
+        if (t.const_data_ptr() != at || (long)t._version() != version) Py_RETURN_FALSE;
+    }
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // x (B,C,H,W) -> (B,C): mean of relu(x) over the pixels
 PyObject *py_relu_mean(PyObject *, PyObject *o)
 {
@@ -1081,6 +1105,7 @@ PyMethodDef methods[] = {
     WG_FN("quantize_int8", py_quantize_int8),
     WG_FN("rms_norm_int8", py_rms_norm_int8),
     WG_FN("linear_int8", py_linear_int8),
+    WG_FN("unchanged", py_unchanged),
     WG_FN("maxpool", py_maxpool),
     WG_FN("stem_pool", py_stem_pool),
     WG_FN("imtrans_op", py_imtrans_op),

@@ -13,11 +13,14 @@ kernels; the other 1x1 shortcuts and the classifier are stock torch ops, or, wit
 stages (56x56 and 28x28) run as one kernel each, BatchNorms and shortcut add included (a shortcut that goes through a ReLU first gets
 it in a pass of its own there, and inside the last kernel elsewhere).  Weights are random (seeded): there is no checkpoint to load here.
 """
+import threading
+
 import numpy as np
 import torch
 import torch.nn.functional as F
 
 import wg2x2
+from wg2x2._native import unchanged
 
 STAGES = ((64, 64), (64, 128), (128, 256), (256, 512))       # (channels in, channels out) per stage
 DENSITY = (0.6, 0.4, 0.3, 0.2)                               # Winograd-domain weight density per stage
@@ -29,6 +32,52 @@ def _same_pool(x):
     padding.  For an odd size it pads one on each side: padding=1."""
     H, W = x.shape[2], x.shape[3]
     return F.max_pool2d(x, 3, 2, padding=(H % 2, W % 2), ceil_mode=True)
+
+
+class _Made(tuple):
+    """Tensors made of weights; `seen`: the weights as they were then (a tensor, one of its memory, which keeps another from having that
+    address, the address, the count of writes).  A copy of the module makes its own: this becomes None in it."""
+
+    seen = ()
+
+    def __reduce__(self):
+        return type(None), ()
+
+
+_making = threading.Lock()
+
+
+def _made(owner, name, make, *weights):
+    """make(*weights), a tuple of tensors that is kept as owner.name while the weights are the same tensors, over the same memory, with
+    nothing written to them.  What has become stale is made anew in the memory that it had, so that captured graphs follow, once the device
+    has done what was asked of it before; and whoever makes something waits until it is there, so that any stream may read it.  A call
+    inside a capture that finds nothing, or something stale, records the making in its graph and keeps nothing; neither is anything kept of weights that were made
+    in inference mode, to which torch counts no writes."""
+    kept = owner.__dict__.get(name)
+    if kept is not None and unchanged(weights, kept.seen):
+        return kept
+    device = weights[0].device
+    with torch.inference_mode(False), torch.no_grad(), torch.cuda.device(device if device.type == "cuda" else -1):
+        if any(t.is_inference() for t in weights) or (device.type == "cuda" and torch.cuda.is_current_stream_capturing()):
+            return make(*weights)
+        with _making:
+            kept = owner.__dict__.get(name)
+            if kept is not None and unchanged(weights, kept.seen):
+                return kept
+            seen = tuple((t, t.detach(), t.data_ptr(), t._version) for t in weights)
+            new = make(*weights)
+            if kept is not None and kept[0].device == device and [s[1].shape for s in kept.seen] == [t.shape for t in weights]:
+                if device.type == "cuda":
+                    torch.cuda.synchronize(device)
+                for there, t in zip(kept, new):
+                    there.copy_(t)
+                new = kept
+            made = _Made(new)
+            made.seen = seen
+            if device.type == "cuda":
+                torch.cuda.current_stream(device).synchronize()
+            owner.__dict__[name] = made
+    return made
 
 
 class _BN(torch.nn.Module):
@@ -152,17 +201,22 @@ class ResNet18Var(torch.nn.Module):
         t = conv(blk["w2b"], blk["bn2b"](t))
         return main + blk["bn2c"](t)
 
-    def _codes_of(self, owner, name, weights):
-        """quantize_int8 of the weights that the call gives, kept on `owner` until they are on another device"""
-        kept = getattr(owner, name, None)
-        if kept is None or kept[0].device != self.fc_w.device:
-            kept = wg2x2.quantize_int8(weights().detach().flatten(1).contiguous())
-            setattr(owner, name, kept)
-        return kept
+    @staticmethod
+    def _codes(w, scale=None):
+        """quantize_int8 of (scaled) weights"""
+        return wg2x2.quantize_int8((w if scale is None else w * scale.view(-1, 1, 1, 1)).flatten(1).contiguous())
+
+    def weights_changed(self):
+        """To be called after writes to weights that torch does not count: through `.data` or an address.  What is kept of them is
+        made anew by the next call outside of a capture.  (Other changes, load_state_dict among them, are seen.)"""
+        for owner in self.modules():
+            for kept in owner.__dict__.values():
+                if isinstance(kept, _Made):
+                    kept.seen = tuple((*s[:3], -1) for s in kept.seen)
 
     def _shortcut_int8(self, blk, x, relu):
         """bn1(conv1x1([relu]x)) in 8 bits, without bn1's shift where the block's last kernel adds it"""
-        w, w_scale = self._codes_of(blk, "_short_codes", lambda: blk.short * blk["bn1"].scale.view(-1, 1, 1, 1))
+        w, w_scale = _made(blk, "_short_codes", self._codes, blk.short, blk["bn1"].scale)
         q, scale = wg2x2.quantize_int8(_WinogradLayer._to_kernel(x, self.layout), relu=relu, layout=self.layout)
         y = wg2x2.linear_int8(q, scale, w, w_scale, bias=None if self.fused else blk["bn1"].shift, layout=self.layout)
         return _WinogradLayer._from_kernel(y, self.layout)
@@ -235,7 +289,7 @@ class ResNet18Var(torch.nn.Module):
             l = torch.relu(l).mean(dim=(2, 3))
         if int8:
             q, scale = wg2x2.quantize_int8(l.contiguous())
-            return wg2x2.linear_int8(q, scale, *self._codes_of(self, "_fc_codes", lambda: self.fc_w), bias=self.fc_b)
+            return wg2x2.linear_int8(q, scale, *_made(self, "_fc_codes", self._codes, self.fc_w), bias=self.fc_b)
         return F.linear(l, self.fc_w, self.fc_b)
 
     def winograd_layers(self):

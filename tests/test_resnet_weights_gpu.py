@@ -1,0 +1,111 @@
+"""ResNet18Var keeps what its kernels take of the weights: it follows the weights, on any stream, and inside and outside of captured graphs."""
+import pytest
+import torch
+
+import resnet18_var
+
+pytestmark = pytest.mark.gpu
+
+
+def _image(seed=1):
+    return torch.randn((2, 3, 64, 64), generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def _net(**how):
+    return resnet18_var.ResNet18Var(num_classes=60, **how).cuda().eval()
+
+
+def _fresh(net, image, **how):
+    """The logits of a network that has never seen other weights"""
+    new = _net(**how)
+    new.load_state_dict(net.state_dict())
+    return new(image)
+
+
+def _scale(t):
+    t.mul_(torch.linspace(0.5, 1.5, t.numel(), device=t.device).view(t.shape))
+
+
+def _pointwise(seed):
+    """Shortcuts and classifier of another network"""
+    return {n: t for n, t in _net(seed=seed, **INT8).state_dict().items() if "short" in n or "bn1" in n or "fc_" in n}
+
+
+INT8 = dict(pointwise="int8", fused=False)
+
+
+@pytest.mark.parametrize("layout", ["NCHW", "NHWC"])
+@pytest.mark.parametrize("name", ["fc_w", "blocks.0.0.short", "blocks.3.0.short", "blocks.1.0.bn1.scale"])
+def test_codes_follow_writes(name, layout):
+    how = dict(INT8, layout=layout)
+    net, image = _net(**how), _image()
+    before = net(image)
+    _scale(net.state_dict()[name])
+    after = net(image)
+    assert not torch.equal(after, before) and torch.equal(after, _fresh(net, image, **how)) and torch.equal(net(image), after)
+
+
+def test_codes_follow_loaded_and_replaced_weights():
+    net, image = _net(**INT8), _image()
+    net(image)
+    net.load_state_dict(_pointwise(5), strict=False)
+    assert torch.equal(net(image), _fresh(net, image, **INT8))
+    net.fc_w = torch.nn.Parameter(torch.randn_like(net.fc_w), requires_grad=False)
+    assert torch.equal(net(image), _fresh(net, image, **INT8))
+    net.fc_w = torch.nn.Parameter(torch.randn((7, 512), device="cuda"), requires_grad=False)        # a head of another size
+    net.fc_b = torch.nn.Parameter(torch.randn(7, device="cuda"), requires_grad=False)
+    assert net(image).shape == (2, 7)
+    net.fc_w.data.mul_(2)                      # (torch counts no such writes)
+    net.weights_changed()
+    net.fc_b.zero_()
+    a = net(image)
+    net.fc_w.mul_(0.5)
+    assert torch.equal(net(image) * 2, a)      # (a power of two: every rounding alike)
+
+
+def test_first_call_on_another_stream():
+    net, image = _net(**INT8), _image()
+    want = _fresh(net, image, **INT8)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(20_000_000)          # (some 10 ms in front of the codes of the weights)
+        net(image)
+    with torch.cuda.stream(b):
+        y = net(image)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
+def test_first_call_inside_a_capture():
+    net, image = _net(**INT8), _image()
+    want = _fresh(net, image, **INT8)          # (also what torch itself sets up)
+    net.pointwise = None
+    net(image)
+    net.pointwise = "int8"                     # (the codes alone are still to be made)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = net(image)
+    assert torch.equal(net(image), want)       # before the graph has run
+    graph.replay()
+    assert torch.equal(y, want)
+
+
+def test_captured_graph_and_changed_weights():
+    """A graph uses what is kept: after a change, the next call outside of a capture renews that where it is"""
+    net, image = _net(**INT8), _image()
+    want = net(image)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = net(image)
+    graph.replay()
+    assert torch.equal(y, want)
+    for other in (5, 6):
+        net.load_state_dict(_pointwise(other), strict=False)
+        want = net(image)
+        junk = [torch.full((1 << 18,), 1e9, device="cuda") for _ in range(20)]        # (into whatever memory has been given back)
+        graph.replay()
+        assert torch.equal(y, want) and torch.equal(want, _fresh(net, image, **INT8))
+        del junk
