@@ -109,3 +109,16 @@ def test_captured_graph_and_changed_weights():
         graph.replay()
         assert torch.equal(y, want) and torch.equal(want, _fresh(net, image, **INT8))
         del junk
+
+
+def test_round_tf32_inside_a_capture():
+    import wg2x2
+    x = torch.randn(1000, device="cuda")
+    x[::7] = float("nan")
+    want = wg2x2.round_tf32(x)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = wg2x2.round_tf32(x)
+    graph.replay()
+    assert torch.equal(y.view(torch.int32), want.view(torch.int32)) and torch.equal(want.isnan(), x.isnan()) and not want[~x.isnan()].view(torch.int32).bitwise_and(0x1FFF).any()
