@@ -97,6 +97,28 @@ class _BN(torch.nn.Module):
         return b["scale"], b["shift"]
 
 
+def _prepare(W):
+    return (wg2x2.prepare_weights(W),)
+
+
+def _stem_prepare(stem):
+    return (wg2x2.stem_prepare(stem.contiguous()),)
+
+
+def _channels_last(stem):
+    return (stem.clone(memory_format=torch.channels_last),)         # (a tensor of its own, also where the stem already is)
+
+
+def _sum(a, b):
+    return (a + b,)
+
+
+def _fold(short, scale):
+    """1x1 weights with the BatchNorm behind them, and the same as tf32 operands"""
+    folded = short * scale.view(-1, 1, 1, 1)
+    return folded, wg2x2.round_tf32(folded)
+
+
 class _WinogradLayer(torch.nn.Module):
     """WinogradImTrans(relu) + WinogradConv with a fixed pruning mask."""
 
@@ -108,13 +130,9 @@ class _WinogradLayer(torch.nn.Module):
         self.register_buffer("W", (w * mask).contiguous())
         self.register_buffer("mask", mask)
         self.cout = cout
-        self._prepared = None
 
     def prepared(self):
-        W = self._buffers["W"]
-        if self._prepared is None or self._prepared.device != W.device:
-            self._prepared = wg2x2.prepare_weights(W)
-        return self._prepared
+        return _made(self, "_prepared", _prepare, self._buffers["W"])[0]
 
     @staticmethod
     def _to_kernel(x, layout):
@@ -186,9 +204,7 @@ class ResNet18Var(torch.nn.Module):
             # both layers, BatchNorms, ReLUs and the shortcut in one call; a shortcut of None is relu(l)
             wa, wb, (s_out, t_out) = blk["w2a"], blk["w2b"], blk["bn2c"].pair()
             if main_bias is not None:
-                if getattr(blk, "_out_shift_folded", None) is None or blk._out_shift_folded.device != t_out.device:
-                    blk._out_shift_folded = (t_out + main_bias).detach()
-                t_out = blk._out_shift_folded
+                t_out = _made(blk, "_out_shift_folded", _sum, t_out, main_bias)[0]
             y = wg2x2.residual_block(wa._to_kernel(l, self.layout), None if main is None else wa._to_kernel(main, self.layout), wa.prepared(),
                                      blk["bn2a"].pair(), wb.prepared(), blk["bn2b"].pair(), (s_out, t_out), wa.cout, layout=self.layout)
             return wa._from_kernel(y, self.layout)
@@ -234,9 +250,7 @@ class ResNet18Var(torch.nn.Module):
         pre = self.blocks[0][0]["pre"]
         l_relu = None
         if own_stem:      # conv1 + pool1 (+ the first shortcut's BNReLU) as one tensor-core kernel
-            if getattr(self, "_stem_prep", None) is None or self._stem_prep.device != image.device:
-                self._stem_prep = wg2x2.stem_prepare(stem.detach().contiguous())
-            l, l_relu = wg2x2.stem7x7s2_pool(image.contiguous(), self._stem_prep, with_relu=True,
+            l, l_relu = wg2x2.stem7x7s2_pool(image.contiguous(), _made(self, "_stem_prep", _stem_prepare, stem)[0], with_relu=True,
                                              relu_scale=pre.scale, relu_shift=pre.shift)
         elif (self.layout == "NHWC" or own_pool) and not reference:
             # the stem runs channels-last (cuDNN's faster form for it); for NCHW activations the first pool reads that
@@ -245,9 +259,7 @@ class ResNet18Var(torch.nn.Module):
             B_, C_, H_, W_ = image.shape
             x = torch.empty((B_, C_, H_ + 5, W_ + 5), dtype=image.dtype, device=image.device, memory_format=torch.channels_last).zero_()
             x[:, :, 2:2 + H_, 2:2 + W_].copy_(image)
-            if getattr(self, "_stem_cl", None) is None or self._stem_cl.device != stem.device:
-                self._stem_cl = stem.detach().contiguous(memory_format=torch.channels_last)
-            l = F.conv2d(x, self._stem_cl, stride=2)
+            l = F.conv2d(x, _made(self, "_stem_cl", _channels_last, stem)[0], stride=2)
         else:
             l = F.conv2d(F.pad(image, (2, 3, 2, 3)), stem, stride=2)
         if own_stem:
@@ -269,12 +281,10 @@ class ResNet18Var(torch.nn.Module):
             elif reference or not self.fused:
                 main = blk_a["bn1"](F.conv2d(main, blk_a.short))
             else:   # the BatchNorm after the 1x1 shortcut folds into its weights (once) and bias
-                if getattr(blk_a, "_short_folded", None) is None or blk_a._short_folded.device != blk_a.short.device:
-                    blk_a._short_folded = (blk_a.short * blk_a["bn1"].scale.view(-1, 1, 1, 1)).detach()
-                    blk_a._short_tf32 = wg2x2.round_tf32(blk_a._short_folded)
                 # (its shift is added by the block's last kernel)
-                y = wg2x2.conv1x1(main, blk_a._short_tf32) if own_1x1 and main.is_contiguous() else None
-                main = F.conv2d(main, blk_a._short_folded) if y is None else y
+                folded, tf32 = _made(blk_a, "_short_folded", _fold, blk_a.short, blk_a["bn1"].scale)
+                y = wg2x2.conv1x1(main, tf32) if own_1x1 and main.is_contiguous() else None
+                main = F.conv2d(main, folded) if y is None else y
             l = self._block(blk_a, l, main, reference, main_bias=None if (reference or not self.fused) else blk_a["bn1"].shift)
             l = self._block(blk_b, l, None, reference)
             l_relu = None
@@ -315,7 +325,6 @@ class ResNet18Var(torch.nn.Module):
                 layer.mask.copy_(m)
                 w = w * m
             layer.W.copy_(w)
-            layer._prepared = None
 
     def winograd_flops(self, batch, size=224):
         """Dense Winograd-domain flops 2*16*P*C*K summed over the 16 layers (independent of the masks)."""

@@ -122,3 +122,75 @@ def test_round_tf32_inside_a_capture():
         y = wg2x2.round_tf32(x)
     graph.replay()
     assert torch.equal(y.view(torch.int32), want.view(torch.int32)) and torch.equal(want.isnan(), x.isnan()) and not want[~x.isnan()].view(torch.int32).bitwise_and(0x1FFF).any()
+
+
+WAYS = [dict(), dict(layout="NHWC"), dict(fused=False), dict(pointwise="int8"), dict(pointwise="int8", layout="NHWC"), dict(pointwise="int8", fused=False)]
+
+
+@pytest.mark.parametrize("how", WAYS, ids=str)
+def test_every_weight_is_followed(how):
+    net, image = _net(**how), _image()
+    y = net(image)
+    names = [n for n in net.state_dict() if not n.endswith("mask")]
+    for name in [n for n in names if n.split(".")[0] != "blocks" or n[7] in "03"]:          # (first and last stage: every kind there is)
+        _scale(net.state_dict()[name]) if name != "fc_b" else net.fc_b.add_(1)
+        before, y = y, net(image)
+        assert not torch.equal(y, before), name
+    assert torch.equal(y, _fresh(net, image, **how))
+    net.load_state_dict(_net(seed=5, **how).state_dict())
+    assert torch.equal(net(image), _fresh(net, image, **how))
+    for name, t in list(net.named_parameters()):
+        owner, last = net.get_submodule(name.rpartition(".")[0]), name.rpartition(".")[2]
+        setattr(owner, last, torch.nn.Parameter(torch.randn_like(t) * t.std(), requires_grad=False))
+    assert torch.equal(net(image), _fresh(net, image, **how))
+
+
+@pytest.mark.parametrize("how", WAYS, ids=str)
+def test_first_call_of_a_network_inside_a_capture(how):
+    net, image = _net(**how), _image()
+    want = _fresh(net, image, **how)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = net(image)
+    assert torch.equal(net(image), want)
+    graph.replay()
+    assert torch.equal(y, want)
+    again = torch.cuda.CUDAGraph()             # (now of what is kept)
+    with torch.cuda.graph(again):
+        y = net(image)
+    for seed in (5, 6):
+        net.load_state_dict(_net(seed=seed, **how).state_dict())
+        want = net(image)
+        again.replay()
+        assert torch.equal(y, want)
+
+
+def test_loaded_winograd_weights_in_a_graph():
+    net, image = _net(), _image()
+    net(image)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = net(image)
+    weights = {n: layer.W.cpu().numpy() * 0.5 for n, layer in net.winograd_layers().items()}
+    net.load_winograd_weights(weights)
+    want = net(image)
+    graph.replay()
+    assert torch.equal(y, want) and torch.equal(want, _fresh(net, image))
+
+
+def test_network_made_in_inference_mode():
+    with torch.inference_mode():
+        net, image = _net(), _image()
+        net(image)
+        net.load_state_dict(_net(seed=5).state_dict())
+        assert torch.equal(net(image), _fresh(net, image))
+
+
+def test_network_of_two_devices_in_turn():
+    """Moved to the CPU and back: made anew there"""
+    net, image = _net(pointwise="int8"), _image()
+    want = net(image)
+    net.cpu().cuda()
+    assert torch.equal(net(image), want)
