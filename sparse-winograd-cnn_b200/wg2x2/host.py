@@ -5,7 +5,7 @@ import os
 
 import torch
 
-from . import ops
+from . import _native, ops
 
 
 def _parse_cpulist(text):
@@ -82,10 +82,10 @@ class HostLayerPipeline:
     def _weights(self, Wt):
         if self.math != "tf32":
             return None
-        key = (Wt.data_ptr(), Wt._version)
-        if self._prepared_for != key:
+        # (the tensor itself is kept: freed, its address could become that of other weights, as often written to)
+        if self._prepared_for is None or not _native.unchanged((Wt,), self._prepared_for):
             self._prepared = ops.prepare_weights(Wt)
-            self._prepared_for = key
+            self._prepared_for = () if Wt.is_inference() else ((Wt, Wt.detach(), Wt.data_ptr(), Wt._version),)
         return self._prepared
 
     def submit(self, x_host, Wt, y_host):
