@@ -40,3 +40,23 @@ def test_weights_of_each_batch(how):
         assert torch.equal(_batch(pipe, x, Wt), y)
         assert torch.equal(_batch(pipe, x, Wt), y)
         del Wt
+
+
+@pytest.mark.parametrize("math", ["tf32", "fp32"])
+def test_weights_let_go_while_they_are_queued(math):
+    B, H, W, C = 2, 8, 8, 32
+    x = torch.randn((B, H, W, C)).pin_memory()
+    pipe = wg2x2.HostLayerPipeline(B, H, W, C, C, layout="NHWC", math=math, chunks=1)
+    value = torch.randn((16, C, C), device="cuda")
+    want = _batch(pipe, x, value)
+    y = torch.empty_like(x).pin_memory()
+    Wt, other = value.clone(), torch.randn((16, C, C), device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(pipe.s_run):
+        torch.cuda._sleep(40_000_000)
+    done = pipe.submit(x, Wt, y)
+    del Wt
+    pipe._weights(other)                                                          # (what the next batch would do)
+    junk = [torch.full((16, C, C), 1e9, device="cuda") for _ in range(50)]        # memory that was given back, on the caller's stream
+    done.synchronize()
+    assert torch.equal(y, want) and len(junk) == 50
