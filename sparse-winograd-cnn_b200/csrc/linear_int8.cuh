@@ -280,7 +280,8 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
         tma_load_2d(dst, &mapA, full_bar(s), kc * kLiChunk, lt * kBlockM);
         tma_load_2d(dst + kBlockM * kLiChunk, &mapB, full_bar(s), kc * kLiChunk, ct * prm.N);
     };
-    // The first tile's loads, as many as there are stages, go out before the rest of the set-up
+    // The first tile's loads, as many as there are stages, go out before the rest of the set-up.  (The next kernel is let in by
+    // warp 1, as soon as every CTA has its tensor memory.)
     if (threadIdx.x == 32 || threadIdx.x == 64)
         asm volatile("prefetch.tensormap [%0];" ::"l"(threadIdx.x == 32 ? &mapA : &mapB) : "memory");
     const int early = prm.drop_load >= 0 ? 0 : min(prm.stages, kend - kbeg);
@@ -291,20 +292,21 @@ linear_int8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_consta
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         int lt, ct;
         li_decode(prm, first, lt, ct);
-        wait_for_previous_kernel(kNumSMs);
+        wait_for_previous_results();
         for (int s = 0; s < early; ++s) load(s, lt, ct, kbeg + s);
     }
     __syncwarp();
     if (warp == 1) {
         tmem_alloc(smem_u32((const void *)tmem_ptr_slot), kTmemCols);
         tmem_relinquish();
+        let_next_kernel_in(kNumSMs);
     }
     tc_fence_before();
     __syncthreads();
     if (SPLIT) cluster_sync_all();                  // (a CTA's shared memory is written by others only once it runs)
     tc_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_slot, 0);
-    if (threadIdx.x != 0) wait_for_previous_kernel(kNumSMs);
+    if (threadIdx.x != 0) wait_for_previous_results();
     bool ok = true;
     // SPLIT: an epilogue thread's lane of the tile, and of its columns (part, part + 4, ... of the CTA's) the lane-th; asked for while the
     // products run

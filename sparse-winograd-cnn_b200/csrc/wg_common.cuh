@@ -207,10 +207,18 @@ inline int launch_status()
 // When the next kernel may come in: at once where this grid is small (max_ctas), else when its CTAs have ended.  Let in
 // early beside a grid that occupies the SMs, the next one's CTAs pile up on those that have room or finish first, and a
 // kernel of only one wave then runs unbalanced (16.8 against 14.4 us for the 64 x 256 x 14 x 14 input transform).
-__device__ __forceinline__ void wait_for_previous_kernel(unsigned max_ctas)
+//
+// A kernel with tensor memory has it before it lets the next one in: a CTA of the next kernel on the same SM could take it otherwise,
+// and wait for this kernel's end while this kernel waits for the tensor memory.
+__device__ __forceinline__ void wait_for_previous_results() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_in(unsigned max_ctas)
 {
     if (gridDim.x * gridDim.y * gridDim.z <= max_ctas) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_previous_kernel(unsigned max_ctas)
+{
+    let_next_kernel_in(max_ctas);
+    wait_for_previous_results();
 }
 // First statement of a kernel that touches global memory only through the given pointers.  The pointers pass through the
 // wait, so that no load from them can be moved in front of it.
