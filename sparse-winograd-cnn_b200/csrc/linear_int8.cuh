@@ -838,6 +838,7 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     f.Q = static_cast<const signed char *>(Q); f.W = static_cast<const signed char *>(W);
     f.q_scale = q_scale; f.w_scale = w_scale; f.bias = bias; f.Y = Y; f.ldq = ldq; f.ldw = ldw; f.ldy = ldy;
     f.C = C; f.K = K; f.HW = nchw ? HW : 0; f.relu = relu != 0;
+    const int drop_load = take_drop_load();         // (also by a product whose kernel has no such load: the hook is of the next call, not of a later one)
     int rc;
     if (type == WG2X2_F32 ? li_small<float>(f, rows, st, &rc) : type == WG2X2_F16 ? li_small<__half>(f, rows, st, &rc) : li_small<__nv_bfloat16>(f, rows, st, &rc)) return rc;
     LiParams p = {};
@@ -854,7 +855,7 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     const int b_rows = p.pair ? p.N / 2 : p.N, stage = (kBlockM + b_rows) * kLiChunk, other = 1024 + kLiCtrl + (p.splits > 1 ? p.N * kBlockM * 4 : 0);
     p.stages = std::min({kLiMaxStages, (kLiSmem - other) / stage, std::max(2, p.splits > 1 ? cdiv(p.chunks, p.splits) : kLiMaxStages)});
     p.spin_limit = wait_limit();
-    p.drop_load = take_drop_load();
+    p.drop_load = drop_load;
     CUtensorMap mapA, mapB;
     const void *A = nchw ? Q : W, *Bop = nchw ? W : Q;
     const long long lda = nchw ? ldq : ldw, ldb = nchw ? ldw : ldq;

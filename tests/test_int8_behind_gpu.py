@@ -29,3 +29,23 @@ def test_products_between_kernels_with_tensor_memory():
         got = [(i, calls[i]()) for i in order[part:part + 100]]
         assert all(torch.equal(y, want[i]) for i, y in got)
     assert wg2x2.last_device_status()[0] == 0
+
+
+@pytest.mark.parametrize("rows,C,K", [(1, 4096, 300), (4, 256, 100), (32, 512, 1000)])
+def test_dropped_load_is_of_the_next_product(rows, C, K):
+    """The hook that makes a wait run out is used up by the next product, also by a small one, which waits for nothing"""
+    from wg2x2._lib import lib
+    q, w = wg2x2.quantize_int8(torch.randn((rows, C), device="cuda")), wg2x2.quantize_int8(torch.randn((K, C), device="cuda"))
+    want = wg2x2.linear_int8(*q, *w)
+    x, w1 = torch.randn((2, 64, 14, 14), device="cuda"), wg2x2.round_tf32(torch.randn((64, 64, 1, 1), device="cuda"))
+    other = wg2x2.conv1x1(x, w1)
+    assert wg2x2.last_device_status()[0] == 0
+    assert lib.wg2x2_set_wait_limit(20000) == 0 and lib.wg2x2_test_drop_load(0) == 0
+    try:
+        assert torch.equal(wg2x2.linear_int8(*q, *w), want)
+        torch.cuda.synchronize()
+        assert torch.equal(wg2x2.conv1x1(x, w1), other) and wg2x2.last_device_status()[0] == 0
+    finally:
+        lib.wg2x2_set_wait_limit(0)
+        lib.wg2x2_test_drop_load(-1)
+        wg2x2.last_device_status()
