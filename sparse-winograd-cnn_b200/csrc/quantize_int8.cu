@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
         }
     } else {
         for (int q0 = wi; q0 < words; q0 += LOOP * share) {
-            float v[LOOP][4], r[LOOP][4];
+            float v[LOOP][4], r[LOOP][4], some = 0.f;         // some: these squares (one by one, a thread's would be up to 750 additions on one sum)
 #pragma unroll
             for (int g = 0; g < LOOP; ++g)
 #pragma unroll
@@ -735,9 +735,10 @@ __global__ void __launch_bounds__(512) nchw_kernel(const RowsParams p)
                         if (have && c < C) h[c * HW] = s;
                         v[g][j] = to_f(s);
                     }
-                    if (SUM) ss = fmaf(v[g][j], v[g][j], ss);
+                    if (SUM) some = fmaf(v[g][j], v[g][j], some);
                     amax = mag_max(amax, SUM ? (c < C ? __fmul_rn(v[g][j], weights[c]) : 0.f) : at_least(v[g][j], low));
                 }
+            ss += some;
         }
     }
     // a pixel's maximum and sum over the warps that share it; each of them adds in the same order
