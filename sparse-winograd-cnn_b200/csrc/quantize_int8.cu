@@ -283,14 +283,17 @@ __device__ __forceinline__ float row_scale(const RowCodes &k)
 {
     return k.live ? __fdiv_rn(k.a, 127.f) : (k.a < kTinyRow ? 0.f : __uint_as_float(0x7fffffffu));
 }
-// scale / sqrt(mean square + eps); ss: the sum of the squares of h, or of kDown * h (where eps counts for nothing)
+// scale / sqrt(mean square + eps); ss: the sum of the squares of h, or of kDown * h
 __device__ __forceinline__ float norm_scale(const RowCodes &k, float ss, int C, float eps, bool down)
 {
     const float scale = row_scale(k);
     if (!k.live) return scale;
     const float mean = __fdiv_rn(ss, (float)C);
-    if (down) return scale > 1.f ? __fdiv_rn(scale * kDown, __fsqrt_rn(mean)) : __fdiv_rn(scale, __fsqrt_rn(mean)) * kDown;
-    return __fdiv_rn(scale, __fsqrt_rn(mean + eps));
+    if (down) {
+        const float root = __fsqrt_rn(mean + eps * kDown * kDown);
+        return scale > 1.f ? __fdiv_rn(scale * kDown, root) : __fdiv_rn(scale, root) * kDown;
+    }
+    return __fdiv_rn(scale, 2.f * __fsqrt_rn(fmaf(0.25f, mean, 0.25f * eps)));         // (of a quarter: the sum of both can leave 32 bits)
 }
 
 // The largest magnitude and the sum over `width` lanes (2 to 32).  By shuffles: the warp's own reduction (__reduce_max_sync), behind the ends

@@ -46,3 +46,15 @@ def test_sum_of_squares(layout, C, dtype, kind):
     tol = 1.01 * (0.5 * (1 + _chain(layout, C, dtype) + 2) + 3) * U
     off = ((s.flatten().double() - want).abs() / want).max().item()
     assert off <= tol, (off / U, tol / U)
+
+
+@pytest.mark.parametrize("layout,C", [("NHWC", 64), ("NHWC", 1001), ("NHWC", 40000), ("NCHW", 64), ("NCHW", 2500), ("NCHW", 9000)])
+def test_large_eps_counts(layout, C):
+    """eps next to a mean square of its size, where their sum leaves 32 bits and where the sum of the squares alone does"""
+    for size, eps in ((1.0, 1e38), (1e18, 1e36), (1.7e19, 3e38), (1.8e19, 3.4e38), (1e19, 3.4e38), (1e20, 3.4e38), (1e18, 3.4e38)):
+        x = (1 + torch.rand((40, C), generator=torch.Generator(device="cuda").manual_seed(C), device="cuda")) * size
+        q, s = wg2x2.rms_norm_int8(x if layout == "NHWC" else x.view(40, C, 1, 1), torch.ones(C, device="cuda"), eps=eps, layout=layout)
+        h = x.double()
+        want = h.amax(1) / 127 / torch.sqrt(h.square().mean(1) + float(torch.tensor(eps, dtype=torch.float32)))
+        tol = 1.01 * (0.5 * (1 + _chain(layout, C, torch.float32) + 2) + 3) * U
+        assert ((s.flatten().double() - want).abs() <= tol * want + 2.0 ** -149).all(), (size, eps)
