@@ -729,6 +729,11 @@ RowView need_rows(const Tensor &t, const char *name)
     if (v.rows && !v.ok) value_error(std::string(name) + " must be rows of a common pitch with their elements side by side");
     return v;
 }
+// A tensor of the caller's has been written to: torch's own functions that saved it say so in their backward pass
+void written(const Tensor &t)
+{
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 std::vector<int64_t> leading(const Tensor &t) { return std::vector<int64_t>(t.sizes().begin(), t.sizes().end() - 1); }
 std::vector<int64_t> with_last(std::vector<int64_t> shape, int64_t n) { shape.push_back(n); return shape; }
 
@@ -820,6 +825,8 @@ PyObject *py_quantize_int8(WG_ARGS)
     {
         WG_NOGIL;
         OnDevice on(x);
+        written(q);
+        written(scale);
         new_outputs(d, x, q, scale);
         check(wg2x2_quantize_int8(x.data_ptr(), type_of(x.scalar_type()), d.ld, q.data_ptr(), pitch16(rows_of(q)), ptr(scale), d.B, (int)d.HW, (int)d.C,
                                   layout, relu, on.stream),
@@ -859,6 +866,9 @@ PyObject *py_rms_norm_int8(WG_ARGS)
     {
         WG_NOGIL;
         OnDevice on(x);
+        written(q);
+        written(scale);
+        written(h);
         new_outputs(d, x, q, scale);
         if (res.defined() && !h.defined()) {
             h = Tensor(at::detail::empty_cuda(x.sizes(), x.scalar_type(), x.device(), std::nullopt));
@@ -914,6 +924,7 @@ PyObject *py_linear_int8(WG_ARGS)
     {
         WG_NOGIL;
         OnDevice on(q);
+        written(y);
         if (!y.defined()) y = Tensor(at::detail::empty_cuda(shape, type, q.device(), std::nullopt));
         const Tensor qa = aligned_codes(q), wa = aligned_codes(w);
         check(wg2x2_linear_int8(qa.data_ptr(), pitch16(rows_of(qa)), cptr(scale), wa.data_ptr(), pitch16(rows_of(wa)), cptr(ws), cptr(bias), relu,
