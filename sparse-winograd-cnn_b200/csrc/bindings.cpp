@@ -667,6 +667,7 @@ Tensor arg_on(PyObject *o, const char *name, const Tensor *with, bool optional =
     const Tensor &t = THPVariable_Unpack(o);
     if (t.layout() != at::kStrided) type_error(std::string(name) + " must be a dense tensor");
     if (with && t.device() != with->device()) value_error(std::string(name) + " must be on the same device as the other tensors");
+    if (t.is_neg()) value_error(std::string(name) + " is a negated view: its values are not those of its memory (resolve_neg())");
     return t;
 }
 Tensor arg_real(PyObject *o, const char *name, const Tensor *with, bool optional = false)

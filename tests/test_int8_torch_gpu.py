@@ -34,3 +34,15 @@ def test_outputs_count_as_written():
         wg2x2.quantize_int8(x, scale_out=s2)
     wg2x2.quantize_int8(x, scale_out=s2)
     assert torch.equal(s2, wg2x2.quantize_int8(x)[1])
+
+
+def test_negated_views_are_refused():
+    """The imaginary part of a conjugate: a view whose values are the negatives of its memory's"""
+    x = torch.randn((5, 1), dtype=torch.complex64, device="cuda").conj().imag
+    assert x.is_neg()
+    with pytest.raises(ValueError, match="negated"):
+        wg2x2.quantize_int8(x)
+    with pytest.raises(ValueError, match="negated"):
+        wg2x2.rms_norm_int8(x.resolve_neg(), torch.ones(1, device="cuda"), residual=x)
+    q, s = wg2x2.quantize_int8(x.resolve_neg())
+    assert torch.equal(q.float().flatten() * s, x.flatten().sign() * 127 * s)
