@@ -350,11 +350,17 @@ int wg2x2_set_wait_limit(long long polls);
 /*
  * Test hooks for the time-out path (they fault and hang nothing).  wg2x2_test_drop_load(n): in the next
  * launch of conv_fwd (row-walk), layer_fwd_fused, conv1x1 or linear_int8, CTA 0's (weight) producer stops before its n-th load, so the
- * MMA issuer's wait for that stage runs out; one-shot, n < 0 disarms.  wg2x2_test_wait_probe: a one-thread
+ * MMA issuer's wait for that stage runs out; one-shot, n < 0 disarms (a product too small for the tensor cores' kernels waits for no load: it uses the
+ * hook up).  wg2x2_test_wait_probe: a one-thread
  * kernel that waits `polls` polls on a barrier nobody arrives on and records `where`.
  */
 int wg2x2_test_drop_load(int nth);
 int wg2x2_test_wait_probe(long long polls, unsigned int where, void *stream);
+/*
+ * How wg2x2_linear_int8 cuts a product of `rows` rows (that is not too small for the tensor cores' kernels) on a GPU that holds at_once[0], [1], [2]
+ * clusters of 2, 4 and 8 CTAs: plan = {columns of a tile, CTAs that share one, 1 for pairs of SMs}.  Calls nothing of CUDA.
+ */
+int wg2x2_test_linear_int8_plan(long long rows, int C, int K, int layout, const int *at_once, int *plan);
 
 #ifdef __cplusplus
 }

@@ -897,6 +897,11 @@ extern "C" int wg2x2_linear_int8(const void *Q, long long ldq, const float *q_sc
     return wg::linear_int8(Q, ldq, q_scale, W, ldw, w_scale, bias, relu, Y, type, ldy, B, HW, C, K, layout, (cudaStream_t)stream);
 }
 
+extern "C" int wg2x2_test_linear_int8_plan(long long rows, int C, int K, int layout, const int *at_once, int *plan)
+{
+    return wg::linear_int8_plan(rows, C, K, layout, at_once, plan);
+}
+
 extern "C" int wg2x2_stem_prepared_floats(void) { return wg::kStWtFloats; }
 
 extern "C" int wg2x2_stem_prepare(const float *W, float *Wp, void *stream) { return wg::stem_prepare(W, Wp, (cudaStream_t)stream); }

@@ -769,35 +769,60 @@ static LiClusters li_clusters()
     return c;
 }
 
-// Columns of a tile, CTAs that share one, and whether pairs of SMs do, by an estimate in clocks.  Operands reach an SM at 55 bytes a
-// clock, one of a pair at 42, all SMs together at 6500 (3400 from memory): more than the products themselves take.  A column of 128 lanes is finished in about 10 clocks and a tile in 600 more, beside the next tile's products where there is one.  CTAs that share a
-// tile: two cluster barriers, and the sums' way between SMs, which is narrow.  Measured in a graph, us, C x K x rows, (N, S) taken / next
-// best / a worse one: 2048 x 8191 x 24 (32, 1) 6.4 / (16, 1) 7.0 / (32, 2) 8.0; 4096 x 4096 x 16 (16, 4) 7.0 / (16, 2) 8.4 / (16, 1) 9.1;
-// 4096 x 4096 x 256 (64, 1) 10.4 / (128, 1) 11.3 / (128, 2) 14.8; 8192 x 1024 x 100 (32, 4) 9.5 / (128, 8) 9.8 / (64, 8) 16.4.
+// Columns of a tile, CTAs that share one, and whether pairs of SMs do, by an estimate in clocks, fitted to 338 products with every plan measured
+// (weights from memory in turn; the plan taken costs 1.0 % more than the fastest on average, over 5 % in 23 of them, at most 20; of 331 others the same).  Operands
+// reach an SM at 59 bytes a clock, one of a pair at 45, all SMs together at 8600 (4350 from memory): more than the products themselves take;
+// the first of them after 1100.  A column of 128 lanes is finished in about 14 clocks and a tile in 680 more, beside the next tile's products
+// where there is one.  CTAs come in at 13 clocks each.  CTAs that share a tile: two cluster barriers, and the sums' way between SMs, which
+// is narrow.  Measured in a graph, us, rows x C x K, (N, S) taken / next best / a worse one:
+//   24 x 2048 x 8191 (32, 1) 7.2 / (16, 1) 7.6 / (32, 2) 9.2          64 x 512 x 8000 (64, 1) 4.1 / (32, 1) 4.5 / (16, 1) 5.9
+//   256 x 4096 x 4096 (64, 1) 10.4 / (128, 1) 11.4 / (256, 1) 15.1    100 x 8192 x 1024 (32, 4) 9.7 / (64, 4) 10.8 / (16, 2) 12.0
+//   16 x 8192 x 1024 (16, 8) 7.2 / (16, 4) 8.6 / (16, 1) 16.0         2000 x 2048 x 2048 (256, 1) 10.1 / pairs 11.5 / (128, 1) 11.8
+//   8192 x 1024 x 1024 (256, 1) 10.8 / pairs 12.3 / (128, 1) 13.2     8192 x 4096 x 4096 pairs 89.2 / (256, 1) 96.0 / (128, 1) 120.7
 static void li_choose(LiParams &p, const LiClusters &clusters)
 {
     double best = 1e300;
     const int lanes = p.lanes;
-    const double from_memory = 128.0 * p.chunks * ((double)lanes + p.cols) / 3400;
+    const double from_memory = 128.0 * p.chunks * ((double)lanes + p.cols) / 4350;
     for (int N = 16; N <= 256; N *= 2) {
         const long long cols = cdiv(p.cols, N), tiles = cols * cdiv(lanes, kBlockM);
-        const double bytes = std::max(from_memory, 128.0 * p.chunks * (double)tiles * (kBlockM + N) / 6500), column = 600 + 10.0 * N;
+        const double bytes = std::max(from_memory, 128.0 * p.chunks * (double)tiles * (kBlockM + N) / 8600), column = 680 + 14.0 * N;
         for (int i = 0; i < 4; ++i) {
             const int S = 1 << i;
             if (S > 1 && (N > 128 || S > p.chunks || tiles > clusters.n[i])) break;
-            const double main = (double)cdiv(p.chunks, S) * 128 * (kBlockM + N) / 55, store = column / S;
-            const double t = std::max(bytes, (double)cdivll(tiles * S, kNumSMs) * std::max(main, store)) + std::min(main, store) + (S > 1 ? 1500 + 90 * N : 0);
+            const double main = 1100 + (double)cdiv(p.chunks, S) * 128 * (kBlockM + N) / 59, store = column / S;
+            const double t = std::max(bytes, (double)cdivll(tiles * S, kNumSMs) * std::max(main, store)) + std::min(main, store) +
+                             13.0 * (double)std::min<long long>(tiles * S, kNumSMs) + (S > 1 ? 3500 + 57 * N : 0);
             if (t < best * 0.999) { best = t; p.N = N; p.splits = S; p.pair = 0; }
         }
-        if (N >= 128 && clusters.n[1] > 0) {
+        if (N == 256 && clusters.n[1] > 0) {          // (pairs with 128 columns: never the fastest by more than measurements differ)
             const long long pairs = cols * cdiv(lanes, 256);
-            const double main = (double)p.chunks * 128 * (kBlockM + N / 2) / 42, two = std::max(from_memory, 128.0 * p.chunks * (double)pairs * (256 + N) / 6500);
-            const double t = std::max(two, (double)cdivll(pairs, clusters.n[1]) * std::max(main, column)) + std::min(main, column) + 1500;
+            const double main = 1100 + (double)p.chunks * 128 * (kBlockM + N / 2) / 45, two = std::max(from_memory, 128.0 * p.chunks * (double)pairs * (256 + N) / 8600);
+            const double t = std::max(two, (double)cdivll(pairs, clusters.n[1]) * std::max(main, column)) + std::min(main, column) +
+                             13.0 * (double)std::min<long long>(2 * pairs, kNumSMs) + 1800;
             if (t < best * 0.999) { best = t; p.N = N; p.splits = 1; p.pair = 1; }
         }
     }
     p.lane_tiles = cdiv(lanes, p.pair ? 256 : kBlockM);
     p.col_tiles = cdiv(p.cols, p.N);
+}
+
+static void li_sides(LiParams &p, bool nchw, long long rows, int C, int K)
+{
+    p.lanes = nchw ? (int)rows : K;
+    p.cols = nchw ? K : (int)rows;
+    p.chunks = cdiv(C, kLiChunk);
+}
+// The choice as a test sees it, on a GPU that holds at_once[0], [1], [2] clusters of 2, 4 and 8 CTAs: {columns of a tile, CTAs that share one, pairs}
+int linear_int8_plan(long long rows, int C, int K, int layout, const int *at_once, int *plan)
+{
+    if (rows < 1 || rows > 0x7fffffffLL - 256 || C < 1 || C > kLiMaxC || K < 1 || K > 0x7fffffff - 256 || (layout != WG2X2_NHWC && layout != WG2X2_NCHW) || !at_once || !plan)
+        return WG2X2_ERR_BAD_ARG;
+    LiParams p = {};
+    li_sides(p, layout == WG2X2_NCHW, rows, C, K);
+    li_choose(p, LiClusters{{0, at_once[0], at_once[1], at_once[2]}});
+    plan[0] = p.N; plan[1] = p.splits; plan[2] = p.pair;
+    return WG2X2_OK;
 }
 
 template <bool NCHW, typename T, bool SPLIT>
@@ -845,9 +870,7 @@ int linear_int8(const void *Q, long long ldq, const float *q_scale, const void *
     p.Y = Y; p.ldy = ldy; p.bias = bias; p.K = K; p.HW = HW; p.relu = relu != 0;
     p.lane_scale = nchw ? q_scale : w_scale;
     p.col_scale = nchw ? w_scale : q_scale;
-    p.lanes = nchw ? (int)rows : K;
-    p.cols = nchw ? K : (int)rows;
-    p.chunks = cdiv(C, kLiChunk);
+    li_sides(p, nchw, rows, C, K);
     const LiClusters clusters = li_clusters();
     li_choose(p, clusters);
     const int pairs = clusters.n[1];

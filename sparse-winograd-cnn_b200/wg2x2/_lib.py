@@ -78,6 +78,7 @@ _SIGS = {
     "wg2x2_last_device_status": (_i, [_p, ctypes.POINTER(ctypes.c_uint)]),
     "wg2x2_set_wait_limit": (_i, [ctypes.c_longlong]),
     "wg2x2_test_drop_load": (_i, [_i]),
+    "wg2x2_test_linear_int8_plan": (_i, [_l, _i, _i, _i, _p, _p]),
     "wg2x2_test_wait_probe": (_i, [ctypes.c_longlong, ctypes.c_uint, _p]),
 }
 for _name, (_res, _args) in _SIGS.items():
