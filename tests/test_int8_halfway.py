@@ -36,5 +36,6 @@ def test_half_way_points_are_among_them():
     a, u = pairs(11)
     twice = 254 * u.astype(np.float64) / a.astype(np.float64)
     half = (twice == np.rint(twice)) & (twice % 2 == 1) & (u <= a)
-    # a / 2 is half way for every a; where a's mantissa is one of the eight multiples of 127, 9 to 16 times it, most odd multiples of a / 254 are values
-    assert (half.sum(1) >= 1).all() and (half.sum(1) > 100).sum() == 8
+    # a / 2 is half way for every a.  Others are where a's mantissa is j times 127, j = 9 .. 16: the j k / 2 that have 11 bits, k odd, for j = 15 those up
+    # to k = 136
+    assert (half.sum(1) >= 1).all() and (half.sum(1) > 1).sum() == 8 and half.sum(1).max() > half.sum(1)[127 * 15 - 1024] == 68
