@@ -695,6 +695,7 @@ static bool li_small_launch(const LiSmallParams &p, cudaStream_t st, int *rc)
 //    more: 32 x 64 x 100 2.1 / 3.9, 32 x 512 x 4096 3.3 / 4.4, 32 x 4096 x 4096 8.5 / 9.6, 128 x 2048 x 1000 4.8 / 6.8, 128 x 4096 x 1000 7.7 /
 //       8.0; behind it 32 x 2048 x 8191 8.8 / 7.5, 256 x 512 x 1000 5.0 / 4.4.  32 x 16 rows a CTA where that is one for nearly every SM, else 32
 //       x 8: 32 x 512 x 1000 2.6 / 2.8 with the wide ones, 32 x 2048 x 4096 5.7 / 6.3 with the narrow
+//    (four pieces at once with eight rows, and two with 32, spill 20 to 36 bytes a thread for the blocks that then run at once; measured so)
 //    one row: see above; in short rows of weights the second kernel is the faster too (1 x 512 x 8191 2.4 / 4.4, 1 x 1024 x 4096 2.3 / 2.8)
 template <typename T>
 static bool li_small(LiSmallParams p, long long rows, cudaStream_t st, int *rc)

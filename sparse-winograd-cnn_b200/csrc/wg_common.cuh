@@ -229,7 +229,8 @@ __device__ __forceinline__ void after_previous_kernel(P &...p)
     (void)std::initializer_list<int>{([](P &q) { asm volatile("" : "+l"(q)::"memory"); }(p), 0)...};
 }
 
-// Dynamic shared memory above 48 KB has to be granted to a kernel, per device and for the whole process.  A kernel may be launched
+// Shared memory above 48 KB, static and dynamic together, has to be granted to a kernel, per device and for the whole process; launches ask for it from
+// 40 KB of dynamic memory on, since no kernel here has more than 8 KB of its own.  A kernel may be launched
 // with other sizes by several threads at once, so a grant is only ever raised: one thread at a time looks at it and sets it.  What a
 // thread has seen granted it need not ask for again.
 inline bool grant_smem(const void *kernel, size_t bytes)

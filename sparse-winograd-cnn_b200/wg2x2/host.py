@@ -98,7 +98,8 @@ class HostLayerPipeline:
         cur = torch.cuda.current_stream(self.device)
         self.s_in.wait_stream(cur)
         self.s_run.wait_stream(cur)
-        Wt.record_stream(self.s_run)          # (the caller may let go of them as soon as this returns)
+        if Wt.is_cuda:
+            Wt.record_stream(self.s_run)      # (the caller may let go of them as soon as this returns)
         with torch.cuda.stream(self.s_run):
             prepared = self._weights(Wt)
         for i, (lo, hi) in enumerate(self.bounds):
