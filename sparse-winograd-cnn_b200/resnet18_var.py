@@ -66,7 +66,8 @@ def _made(owner, name, make, *weights):
                 return kept
             seen = tuple((t, t.detach(), t.data_ptr(), t._version) for t in weights)
             new = make(*weights)
-            if kept is not None and kept[0].device == device and [s[1].shape for s in kept.seen] == [t.shape for t in weights]:
+            kind = lambda ts: [(t.shape, t.dtype, t.device) for t in ts]  # noqa: E731
+            if kept is not None and kind(kept) == kind(new) and kind(s[1] for s in kept.seen) == kind(weights):
                 if device.type == "cuda":
                     torch.cuda.synchronize(device)
                 for there, t in zip(kept, new):
@@ -226,7 +227,7 @@ class ResNet18Var(torch.nn.Module):
         """To be called after writes to weights that torch does not count: through `.data` or an address.  What is kept of them is
         made anew by the next call outside of a capture.  (Other changes, load_state_dict among them, are seen.)"""
         for owner in self.modules():
-            for kept in owner.__dict__.values():
+            for kept in list(owner.__dict__.values()):
                 if isinstance(kept, _Made):
                     kept.seen = tuple((*s[:3], -1) for s in kept.seen)
 

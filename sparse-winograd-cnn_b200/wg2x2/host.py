@@ -94,7 +94,7 @@ class HostLayerPipeline:
         overlap the kernels and the read-back of this one, so that in steady state the PCIe link is busy in both
         directions all the time.  Device buffers are reused across calls; the event dependencies below keep a
         chunk's buffers from being overwritten while the previous batch still uses them.  The caller must not
-        reuse y_host (or change x_host) before the returned event has completed."""
+        reuse y_host (or change x_host, or write to Wt) before the returned event has completed."""
         cur = torch.cuda.current_stream(self.device)
         self.s_in.wait_stream(cur)
         self.s_run.wait_stream(cur)

@@ -130,3 +130,13 @@ def test_made_in_inference_mode_renewed_outside():
         assert o.right()
     o.w.mul_(3)
     assert o.right() and not o.get()[0].is_inference()
+
+
+def test_other_types_are_made_in_memory_of_their_own():
+    o = _Owner()
+    before = o.get()
+    copied = before[0].clone()
+    o.double()
+    assert o.right() and o.get()[0].dtype == torch.float64 and torch.equal(before[0], copied)
+    o.float()
+    assert o.right() and o.get()[0].dtype == torch.float32
